@@ -1,0 +1,379 @@
+"""The calls of the normalisation, routing and integer-product entry points whose time is measured.
+
+Sizes are those of the model that the backend serves (dim 4096, query latent
+1024 beside a key/value latent of 512, expert inner size 2048, 256 experts of
+which a token takes 6 or 8, attention projections [32768, 1024] and
+[4096, 8192]); token counts run from one decoded token to a long prefill batch.
+Kinds of case:
+
+norm     apus_hip_rmsnorm_dev: residual addition, RMS norm, 8-bit codes.
+route    apus_hip_route_dev: router logits to expert ids and weights.
+product  apus_hip_i8_gemm_dev: 8-bit integer codes times 8-bit integer weights.
+linear   apus_hip_i8_linear_dev: fp32 activations in, quantised per token, product.
+
+run() gives the plain forms in elementary operations, or, where `own` is set,
+makes the calls. Codes come back as what they hold: E4M3 values or integers,
+with their scales beside them.
+"""
+import ctypes as C
+import math
+import os
+import sys
+
+import numpy as np
+import torch
+
+own = False
+
+_PKG = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "apus-deepseek-v4-flash_amd")
+DIM, INTER, EXPERTS = 4096, 2048, 256
+Q_LATENT, KV_LATENT = 1024, 512
+EPS = float(np.float32(1e-6))
+I8_FLOOR = 2.0 ** -100
+
+
+def listed():
+    return [
+        # one decoded token: the norm before a block's FP8 projections
+        {"name": "norm_1", "kind": "norm", "rows": 1, "K": DIM, "ldx": DIM, "bf16": True, "res": True,
+         "y": False, "quant": "e4m3"},
+        # batched decode: the query latent, a slice of the fused query/key-value projection's rows
+        {"name": "norm_100", "kind": "norm", "rows": 100, "K": Q_LATENT, "ldx": Q_LATENT + KV_LATENT,
+         "bf16": False, "res": False, "y": False, "quant": "i8"},
+        # a ragged prompt: the norm before a MoE sublayer (rows for the gate, codes for the experts)
+        {"name": "norm_1000", "kind": "norm", "rows": 1000, "K": DIM, "ldx": DIM, "bf16": False, "res": True,
+         "y": True, "quant": "e4m3"},
+        # a large prefill batch, BF16 residual stream, integer projections behind it
+        {"name": "norm_16384", "kind": "norm", "rows": 16384, "K": DIM, "ldx": DIM, "bf16": True, "res": True,
+         "y": True, "quant": "i8"},
+        # batched decode of 64 sequences, sigmoid scores with a balance bias, 4 of 8 groups
+        {"name": "route_64", "kind": "route", "tokens": 64, "E": EXPERTS, "topk": 8, "score": "sigmoid",
+         "bias": True, "groups": 8, "keep": 4, "top": 2, "scores": False},
+        # a prompt's prefill chunk, softmax over all experts
+        {"name": "route_4095", "kind": "route", "tokens": 4095, "E": EXPERTS, "topk": 6, "score": "softmax",
+         "bias": False, "groups": 1, "keep": 1, "top": 1, "scores": False},
+        # a large prefill batch, the scores kept for the balance statistics
+        {"name": "route_32768", "kind": "route", "tokens": 32768, "E": EXPERTS, "topk": 8, "score": "sigmoid",
+         "bias": True, "groups": 8, "keep": 4, "top": 2, "scores": True},
+        # one decoded token through the attention output projection
+        {"name": "product_1", "kind": "product", "rows": 1, "O": 4096, "K": 8192, "out": "bf16"},
+        # batched decode of 40 sequences: the query projection
+        {"name": "product_40", "kind": "product", "rows": 40, "O": 32768, "K": 1024, "out": "f32"},
+        # a prefill chunk against gate and up projections together
+        {"name": "product_4096", "kind": "product", "rows": 4096, "O": 8192, "K": 4096, "out": "bf16"},
+        # one decoded token, activations quantised in the call
+        {"name": "linear_1", "kind": "linear", "rows": 1, "O": Q_LATENT, "K": DIM, "out": "f32"},
+        # a ragged prompt through the attention output projection
+        {"name": "linear_1000", "kind": "linear", "rows": 1000, "O": 4096, "K": 8192, "out": "bf16"},
+    ]
+
+
+def _log_int(rng, lo, hi):
+    return min(hi, max(lo, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def draw(rng):
+    kind = rng.choice(("norm", "route", "product", "linear"))
+    if kind == "norm":
+        quant = rng.choice(("e4m3", "e4m3", "i8", "i8", "none"))
+        # E4M3 codes have one scale per 128 columns; the others take any row length
+        K = 128 * _log_int(rng, 1, 64) if quant == "e4m3" or rng.random() < 0.5 else _log_int(rng, 32, 8192)
+        bf16 = rng.random() < 0.5
+        most = 16384 * DIM // K // (1 if bf16 else 2)
+        return {"kind": kind, "rows": _log_int(rng, 1, min(32768, most)), "K": K,
+                "ldx": K + rng.choice((0, 0, 8, 512, 5)), "bf16": bf16, "res": rng.random() < 0.6,
+                "y": quant == "none" or rng.random() < 0.4, "quant": quant}
+    if kind == "route":
+        groups = rng.choice((1, 1, 4, 8, 16))
+        E = groups * max(2, _log_int(rng, 8, 512) // groups)
+        keep = rng.randint(1, groups)
+        return {"kind": kind, "tokens": _log_int(rng, 1, 32768 * 256 // max(E, 256)), "E": E,
+                "topk": min(rng.choice((1, 2, 4, 6, 8, 8)), E // groups * keep),
+                "score": rng.choice(("softmax", "sigmoid", "softplus")), "bias": rng.random() < 0.6,
+                "groups": groups, "keep": keep, "top": rng.choice((1, 2)), "scores": rng.random() < 0.3}
+    O, K = _log_int(rng, 16, 32768), 16 * _log_int(rng, 4, 512)
+    if rng.random() < 0.5:
+        O = min(32768, (O + 127) // 128 * 128)
+        K = min(8192, (K + 127) // 128 * 128)
+    most = 4096 * 8192 * 4096 // (O * K)
+    return {"kind": kind, "rows": _log_int(rng, 1, max(1, min(4096, most))), "O": O, "K": K,
+            "out": rng.choice(("f32", "bf16"))}
+
+
+# ------------------------------------------------------------------- inputs
+
+
+def _gen(seed, what):
+    return torch.Generator(device="cuda").manual_seed((seed * 1000003 + what) & 0x7FFFFFFF)
+
+
+def _weight_codes(gen, O, K):
+    """integer weights of N(0, 1) rows scaled to their largest value, and the channels' scales"""
+    w = torch.randn(O, K, device="cuda", generator=gen)
+    a = w.abs().amax(1, keepdim=True)
+    return (w * (127.0 / a)).round().to(torch.int8), a[:, 0] / 127.0 / math.sqrt(K)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def prepare(case, seed):
+    st = {"case": dict(case), "call": None}
+    kind = case["kind"]
+    if kind == "norm":
+        g = _gen(seed, 1)
+        M, K, t = case["rows"], case["K"], torch.bfloat16 if case["bf16"] else torch.float32
+        # a residual stream: channels of different size, rows of different size
+        size = torch.exp(0.5 * torch.randn(1, case["ldx"], device="cuda", generator=g))
+        st["x"] = (torch.randn(M, case["ldx"], device="cuda", generator=g) * size).to(t)
+        st["res"] = (4 * torch.randn(M, K, device="cuda", generator=g)).to(t) if case["res"] else None
+        st["gamma"] = 1 + 0.2 * torch.randn(K, device="cuda", generator=g)
+        st["res_out"] = torch.zeros(M, K, dtype=t, device="cuda") if case["res"] else None
+        st["y"] = torch.zeros(M, K, dtype=t, device="cuda") if case["y"] else None
+        e4 = case["quant"] == "e4m3"
+        st["codes"] = None if case["quant"] == "none" else torch.zeros(
+            M, K, dtype=torch.float8_e4m3fn if e4 else torch.int8, device="cuda")
+        st["scales"] = None if case["quant"] == "none" else torch.zeros(
+            (M, K // 128) if e4 else (M,), device="cuda")
+        return st
+    if kind == "route":
+        g = _gen(seed, 2)
+        s, E, k = case["tokens"], case["E"], case["topk"]
+        # logits of a trained gate: some experts more popular than others
+        st["logits"] = 1.5 * torch.randn(s, E, device="cuda", generator=g) + torch.randn(1, E, device="cuda", generator=g)
+        st["bias"] = 0.05 * torch.randn(E, device="cuda", generator=g) if case["bias"] else None
+        st["idx"] = torch.zeros(s, k, dtype=torch.int32, device="cuda")
+        st["wgt"] = torch.zeros(s, k, device="cuda")
+        st["scores"] = torch.zeros(s, E, device="cuda") if case["scores"] else None
+        return st
+    g = _gen(seed, 3)
+    M, O, K = case["rows"], case["O"], case["K"]
+    st["w"], st["ws"] = _weight_codes(g, O, K)
+    x = torch.randn(M, K, device="cuda", generator=g) * torch.exp(0.5 * torch.randn(1, K, device="cuda", generator=g))
+    st["out"] = torch.zeros(M, O, dtype=torch.bfloat16 if case["out"] == "bf16" else torch.float32, device="cuda")
+    if kind == "linear":
+        st["x"] = x.bfloat16().float()
+        st["space"] = torch.empty((M * K + 255) // 256 * 256 + (4 * M + 255) // 256 * 256, dtype=torch.uint8, device="cuda")
+        return st
+    a = x.abs().amax(1, keepdim=True)
+    st["a"], st["as"] = (x * (127.0 / a)).round().to(torch.int8), a[:, 0] / 127.0
+    return st
+
+
+# -------------------------------------------------------------- plain forms
+
+
+def _pow2(e):
+    return (e << 23).view(torch.float32)
+
+
+def _quant_e4m3(b):
+    """power-of-two scale of each 128 columns and the E4M3 values under it, of BF16-valued b [M, K]"""
+    v = b.view(b.shape[0], -1, 128)
+    p = (v.abs().amax(2).clamp_min(1e-4) * (1.0 / 448.0)).view(torch.int32)
+    e = (p >> 23) + ((p & 0x7FFFFF) != 0).to(torch.int32)
+    codes = (v * _pow2(254 - e)[:, :, None]).to(torch.float8_e4m3fn)
+    return codes.view(b.shape), _pow2(e)
+
+
+def _quant_i8(b):
+    """scale of each row (its largest value / 127) and the integers under it, of BF16-valued b [M, K]"""
+    a = b.abs().amax(1).double().clamp_min(I8_FLOOR)
+    inv = torch.div(torch.full_like(a, 127.0), a).float()
+    q = (b * inv[:, None]).round().clamp(-127, 127)
+    return q.to(torch.int8), (a / 127.0).float()
+
+
+def _norm(st):
+    case = st["case"]
+    t, K = st["x"].dtype, case["K"]
+    r = st["x"][:, :K].float()
+    out = {}
+    if case["res"]:
+        out["res_out"] = (r + st["res"].float()).to(t)
+        r = out["res_out"].float()
+    # 64 bits: the codes behind it hang on which side of a rounding border a value lies
+    d = r.double()
+    inv = 1.0 / torch.sqrt(d.square().sum(1, keepdim=True) / K + EPS)
+    y = (d * st["gamma"].double() * inv).float()
+    if case["y"]:
+        out["y"] = y.to(t)
+    if case["quant"] != "none":
+        b = y.bfloat16().float()
+        out["codes"], out["scales"] = _quant_e4m3(b) if case["quant"] == "e4m3" else _quant_i8(b)
+    return out
+
+
+def _route(st):
+    case = st["case"]
+    s, E, k, G = case["tokens"], case["E"], case["topk"], case["groups"]
+    # 64 bits: two experts' scores next to each other decide which one is chosen
+    z = st["logits"].double()
+    if case["score"] == "softmax":
+        p = torch.exp(z - z.amax(1, keepdim=True))
+        p = p / p.sum(1, keepdim=True)
+    elif case["score"] == "sigmoid":
+        p = 1.0 / (1.0 + torch.exp(-z))
+    else:
+        p = torch.sqrt(z.clamp_min(0) + torch.log1p(torch.exp(-z.abs())))
+    sel = p + st["bias"].double() if case["bias"] else p
+    if G > 1:
+        each = sel.view(s, G, E // G)
+        best = torch.sort(each, dim=2, descending=True).values[:, :, :case["top"]].sum(2)
+        kept = torch.sort(best, dim=1, descending=True, stable=True).indices[:, :case["keep"]]
+        mask = torch.zeros(s, G, dtype=torch.bool, device=sel.device).scatter_(1, kept, True)
+        sel = torch.where(mask[:, :, None], each, -math.inf).view(s, E)
+    idx = torch.sort(sel, dim=1, descending=True, stable=True).indices[:, :k]
+    w = torch.gather(p, 1, idx)
+    w = w / w.sum(1, keepdim=True) * 2.5
+    out = {"idx": idx.to(torch.int32), "wgt": w.float()}
+    if case["scores"]:
+        out["scores"] = p.float()
+    return out
+
+
+def _product(a, sa, w, sb, t):
+    acc = a.float() @ w.float().t()
+    return (acc * sa[:, None] * sb[None, :]).to(t)
+
+
+def _plain(st):
+    kind = st["case"]["kind"]
+    if kind == "norm":
+        return _norm(st)
+    if kind == "route":
+        return _route(st)
+    if kind == "product":
+        return {"out": _product(st["a"], st["as"], st["w"], st["ws"], st["out"].dtype)}
+    q, s = _quant_i8(st["x"].bfloat16().float())
+    return {"out": _product(q, s, st["w"], st["ws"], st["out"].dtype)}
+
+
+# --------------------------------------------------------- the entry points
+
+
+def _call(st):
+    """The entry point of this state and its arguments, put together once."""
+    if _PKG not in sys.path:
+        sys.path.insert(0, _PKG)
+    import apus_hip as H
+    H.enable()
+    L, case, kind = H.lib(), st["case"], st["case"]["kind"]
+    if kind == "norm":
+        flags = (H.X_BF16 | H.Y_BF16 if case["bf16"] else 0) | (H.Q_I8 if case["quant"] == "i8" else 0)
+        args = (_ptr(st["x"]), case["ldx"], _ptr(st["res"]), _ptr(st["res_out"]), _ptr(st["gamma"]), case["rows"],
+                case["K"], EPS, flags, _ptr(st["y"]), _ptr(st["codes"]), _ptr(st["scales"]))
+        return H, L.apus_hip_rmsnorm_dev, args, {n: st[n] for n in ("res_out", "y", "codes", "scales") if st[n] is not None}
+    if kind == "route":
+        score = {"softplus": H.SCORE_SQRTSOFTPLUS, "sigmoid": H.SCORE_SIGMOID, "softmax": H.SCORE_SOFTMAX}[case["score"]]
+        cfg = st["cfg"] = H.ApusHipRoute(score, case["topk"], case["groups"], case["keep"], case["top"], 1, 2.5)
+        args = (C.byref(cfg), _ptr(st["logits"]), _ptr(st["bias"]), case["tokens"], case["E"], _ptr(st["idx"]),
+                _ptr(st["wgt"]), _ptr(st["scores"]))
+        return H, L.apus_hip_route_dev, args, {n: st[n] for n in ("idx", "wgt", "scores") if st[n] is not None}
+    flags = H.Y_BF16 if case["out"] == "bf16" else 0
+    if kind == "product":
+        args = (_ptr(st["w"]), _ptr(st["ws"]), _ptr(st["a"]), _ptr(st["as"]), _ptr(st["out"]), case["rows"], case["O"],
+                case["K"], flags)
+        return H, L.apus_hip_i8_gemm_dev, args, {"out": st["out"]}
+    args = (_ptr(st["w"]), _ptr(st["ws"]), _ptr(st["x"]), _ptr(st["out"]), case["rows"], case["K"], case["O"],
+            flags, _ptr(st["space"]))
+    return H, L.apus_hip_i8_linear_dev, args, {"out": st["out"]}
+
+
+def run(state):
+    if not own:
+        return _plain(state)
+    if state["call"] is None:
+        state["call"] = _call(state)
+    H, entry, args, out = state["call"]
+    H._check(entry(*args), state["case"]["kind"])
+    return out
+
+
+# --------------------------------------------------------------------- work
+
+
+def work(case):
+    kind = case["kind"]
+    if kind == "norm":
+        n, M, K, e = case["rows"] * case["K"], case["rows"], case["K"], 2 if case["bf16"] else 4
+        q = 0 if case["quant"] == "none" else n + 4 * (n // 128 if case["quant"] == "e4m3" else M)
+        return {"bytes": n * e * (1 + 2 * case["res"] + case["y"]) + 4 * K + q, "flops": 6 * n}
+    if kind == "route":
+        s, E = case["tokens"], case["E"]
+        return {"bytes": 4 * s * E * (1 + case["scores"]) + 8 * s * case["topk"] + 4 * E * case["bias"], "flops": 8 * s * E}
+    M, O, K = case["rows"], case["O"], case["K"]
+    acts = M * (K + 4) if kind == "product" else 4 * M * K
+    return {"bytes": O * (K + 4) + acts + M * O * (2 if case["out"] == "bf16" else 4), "flops": 2 * M * O * K}
+
+
+# -------------------------------------------------------------------- exact
+
+
+def _bf16(v):
+    """64-bit values through fp32 to BF16, ties to even, on the bits"""
+    u = np.ascontiguousarray(v.astype(np.float32)).view(np.uint32).astype(np.uint64)
+    u = (u + 0x7FFF + ((u >> 16) & 1)) & 0xFFFF0000
+    return u.astype(np.uint32).view(np.float32).astype(np.float64)
+
+
+def _host(t):
+    return t.detach().double().cpu().numpy()
+
+
+def exact(case, seed):
+    st = prepare(case, seed)
+    kind = case["kind"]
+    if kind == "norm":
+        K, out = case["K"], {}
+        r = _host(st["x"])[:, :K]
+        if case["res"]:
+            r = r + _host(st["res"])
+            out["res_out"] = r = _bf16(r) if case["bf16"] else r.astype(np.float32).astype(np.float64)
+        y = r / np.sqrt(np.einsum("mk,mk->m", r, r) / K + EPS)[:, None] * _host(st["gamma"])
+        if case["y"]:
+            out["y"] = y
+        if case["quant"] != "none":
+            b, out["codes"] = np.abs(_bf16(y)), None
+            if case["quant"] == "e4m3":
+                top = np.maximum(b.reshape(len(b), -1, 128).max(2), np.float64(np.float32(1e-4)))
+                p = (top.astype(np.float32) * np.float32(1.0 / 448.0)).astype(np.float64)
+                out["scales"] = 2.0 ** np.ceil(np.log2(p))
+            else:
+                out["scales"] = np.maximum(b.max(1), I8_FLOOR) / 127.0
+        return out
+    if kind == "route":
+        z, s, E = _host(st["logits"]), case["tokens"], case["E"]
+        if case["score"] == "softmax":
+            m = z.max(1, keepdims=True)
+            p = np.exp(z - m - np.log(np.exp(z - m).sum(1, keepdims=True)))
+        elif case["score"] == "sigmoid":
+            p = 0.5 * (1.0 + np.tanh(0.5 * z))
+        else:
+            p = np.sqrt(np.logaddexp(0.0, z))
+        sel = p + (_host(st["bias"]) if case["bias"] else 0.0)
+        rows = np.arange(s)[:, None]
+        if case["groups"] > 1:
+            per = E // case["groups"]
+            best = -np.sort(-sel.reshape(s, -1, per), axis=2)[:, :, :case["top"]].sum(2)
+            out_of = np.argsort(-best, axis=1, kind="stable")[:, case["keep"]:]
+            sel = sel.reshape(s, -1, per).copy()
+            sel[rows, out_of] = -np.inf
+            sel = sel.reshape(s, E)
+        idx = np.argsort(-sel, axis=1, kind="stable")[:, :case["topk"]]
+        w = p[rows, idx]
+        out = {"idx": None, "wgt": 2.5 * w / w.sum(1, keepdims=True)}
+        if case["scores"]:
+            out["scores"] = p
+        return out
+    if kind == "product":
+        a, sa = st["a"], st["as"]
+    else:
+        b = _bf16(_host(st["x"]))
+        top = np.maximum(np.abs(b).max(1), I8_FLOOR)
+        q = np.rint(b.astype(np.float32) * (127.0 / top).astype(np.float32)[:, None])
+        a, sa = torch.from_numpy(q).cuda(), torch.from_numpy((top / 127.0).astype(np.float32)).cuda()
+    # sums of integers below 2^53: exact
+    acc = torch.matmul(st["w"].double(), a.double().t().contiguous())
+    return {"out": (acc * st["ws"].double()[:, None] * sa.double()[None, :]).t().contiguous()}
