@@ -23,6 +23,9 @@ import numpy as np
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libapus_hip.so")
 W_TILED = 0x100        # APUS_HIP_W_TILED: weights in the MFMA-tiled layout
+# flags of the norm and integer entry points (APUS_HIP_*)
+R_OUT, W_BF16, X_BF16, Y_BF16, Q_I8 = 2, 4, 8, 16, 32
+SCORE_SQRTSOFTPLUS, SCORE_SIGMOID, SCORE_SOFTMAX = 0, 1, 2
 
 u8p = C.POINTER(C.c_uint8)
 f32p = C.POINTER(C.c_float)
@@ -90,6 +93,13 @@ class ApusHipMoeInterm(C.Structure):
     _fields_ = [("router_scores", vp), ("router_idx", vp), ("router_w", vp),
                 ("moe_routed", vp), ("moe_shared", vp)]
 
+
+class ApusHipRoute(C.Structure):
+    """Expert choice of apus_hip_route_dev (include/apus_hip.h)."""
+    _fields_ = [("score", C.c_int), ("topk", C.c_int), ("n_group", C.c_int), ("topk_group", C.c_int),
+                ("group_top", C.c_int), ("renorm", C.c_int), ("route_scale", C.c_float)]
+
+
 class ApusHipSlabRec(C.Structure):
     """One routed expert's slab in an apus container (include/apus_hip.h)."""
     _fields_ = [("shard", C.c_int32), ("pad", C.c_int32), ("off", C.c_uint64), ("len", C.c_uint64),
@@ -148,6 +158,13 @@ SIGNATURES = {
     "apus_hip_moe_forward_dev": (C.c_int, [vp, C.c_int, C.POINTER(ApusHipMoeLayer), vp, vp,
                                            C.c_int, C.c_int, vp, C.POINTER(ApusHipMoeInterm),
                                            vp]),
+    "apus_hip_rmsnorm_dev": (C.c_int, [vp, C.c_int, vp, vp, vp, C.c_int, C.c_int, C.c_float, C.c_int,
+                                       vp, vp, vp]),
+    "apus_hip_route_dev": (C.c_int, [C.POINTER(ApusHipRoute), vp, vp, C.c_int, C.c_int, vp, vp, vp]),
+    "apus_hip_i8_quant_dev": (C.c_int, [vp, C.c_int, C.c_int, C.c_int, vp, vp]),
+    "apus_hip_i8_gemm_dev": (C.c_int, [vp, vp, vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int]),
+    "apus_hip_i8_linear_workspace": (C.c_size_t, [C.c_int, C.c_int]),
+    "apus_hip_i8_linear_dev": (C.c_int, [vp, vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, vp]),
     "apus_hip_container_open": (vp, [C.c_char_p, C.c_int, C.c_int, C.c_int, C.c_char_p,
                                      C.c_size_t]),
     "apus_hip_container_close": (None, [vp]),

@@ -1325,6 +1325,204 @@ int apus_hip_fp8_linear_dev(const uint8_t *w, const uint8_t *ws, const float *x,
     return linear_dev(APUS_W_FP8, w, ws, x, out, M, K, O, workspace);
 }
 
+/* ---- norm, routing, integer products ---- */
+
+namespace {
+
+/* The launches go to streams of device 0: it is the current device while an
+ * entry point runs, whatever the caller's is. */
+struct OnDevice0 {
+    int prev = 0;
+    OnDevice0() {
+        if (hipGetDevice(&prev) != hipSuccess) prev = 0;
+        if (prev != 0) (void)hipSetDevice(0);
+    }
+    ~OnDevice0() {
+        if (prev != 0) (void)hipSetDevice(prev);
+    }
+};
+
+struct Span {
+    const void *p;
+    size_t n;
+};
+
+bool overlap(const Span &a, const Span &b) {
+    if (!a.p || !b.p) return false;
+    const uintptr_t x = (uintptr_t)a.p, y = (uintptr_t)b.p;
+    return x < y + b.n && y < x + a.n;
+}
+
+bool aligned(const void *p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+
+/* the kernels round row and column counts up to their tiles in 32 bits */
+constexpr int ROWS_LIMIT = 0x7fffff00;
+
+bool no_overlap(const Span *out, int n_out, const Span *in, int n_in, const char *what) {
+    for (int i = 0; i < n_out; i++) {
+        for (int j = i + 1; j < n_out; j++)
+            if (overlap(out[i], out[j])) { set_err("%s: two outputs overlap", what); return false; }
+        for (int j = 0; j < n_in; j++)
+            if (overlap(out[i], in[j])) { set_err("%s: an output overlaps an input", what); return false; }
+    }
+    return true;
+}
+
+bool i8_args_ok(const void *w, const void *ws, const void *x, const void *out, int M, int O, int K, int flags,
+                int allowed, const char *what) {
+    if (M < 0 || O <= 0 || K <= 0 || K % 4 || K > 131068 || M > ROWS_LIMIT || O > ROWS_LIMIT) {
+        set_err("%s: unsupported shape M=%d O=%d K=%d (needs K %% 4 == 0, K <= 131068)", what, M, O, K);
+        return false;
+    }
+    if (flags & ~allowed) { set_err("%s: unknown flags %#x", what, flags & ~allowed); return false; }
+    if (!w || !ws || !x || !out || !aligned(w, 4) || !aligned(ws, 4) ||
+        !aligned(x, (allowed & APUS_HIP_X_BF16) && (flags & APUS_HIP_X_BF16) ? 2 : 4) ||
+        !aligned(out, flags & APUS_HIP_Y_BF16 ? 2 : 4)) {
+        set_err("%s: null or misaligned array", what);
+        return false;
+    }
+    return true;
+}
+
+}  // namespace
+
+int apus_hip_rmsnorm_dev(const void *x, int ldx, const void *res, void *res_out, const void *gamma, int M, int K,
+                         float eps, int flags, void *y, uint8_t *codes, float *scales) {
+    const bool xb = flags & APUS_HIP_X_BF16, yb = flags & APUS_HIP_Y_BF16, i8 = flags & APUS_HIP_Q_I8;
+    const size_t ex = xb ? 2 : 4, ey = yb ? 2 : 4, eg = flags & APUS_HIP_W_BF16 ? 2 : 4;
+    if (flags & ~(APUS_HIP_R_OUT | APUS_HIP_W_BF16 | APUS_HIP_X_BF16 | APUS_HIP_Y_BF16 | APUS_HIP_Q_I8)) {
+        set_err("rmsnorm: unknown flags %#x", flags);
+        return 1;
+    }
+    if (M < 0 || K <= 0 || ldx < K || M > ROWS_LIMIT || K > ROWS_LIMIT || (codes && !i8 && K % 128)) {
+        set_err("rmsnorm: unsupported shape M=%d K=%d ldx=%d (E4M3 codes need K %% 128 == 0)", M, K, ldx);
+        return 1;
+    }
+    if (!(eps > 0.0f) || eps == __builtin_inff()) { set_err("rmsnorm: eps must be positive and finite"); return 1; }
+    if (!x || !gamma || (!y && !codes && !res_out) || !codes != !scales || (res_out && !res)) {
+        set_err("rmsnorm: x and gamma are needed, an output, scales with codes, and res with res_out");
+        return 1;
+    }
+    if (!aligned(x, ex) || !aligned(res, ex) || !aligned(res_out, ex) || !aligned(gamma, eg) || !aligned(y, ey) ||
+        !aligned(scales, 4)) {
+        set_err("rmsnorm: misaligned array");
+        return 1;
+    }
+    if (M == 0) return 0;
+    const size_t n = (size_t)M * K;
+    const Span sx{x, ((size_t)(M - 1) * ldx + K) * ex}, sr{res, n * ex}, sg{gamma, (size_t)K * eg};
+    const Span so{res_out, n * ex}, sy{y, n * ey}, sc{codes, n}, ss{scales, (i8 ? (size_t)M : n / 128) * 4};
+    /* in place: an element of these outputs is written by the thread that read
+     * the input's, after the row's last use of it */
+    const bool dense = ldx == K;
+    const bool o_in_x = dense && res_out == x, o_in_r = res_out == res;
+    const bool y_in_x = dense && ex == ey && y == x, y_in_r = ex == ey && y && y == res;
+    const Span none{nullptr, 0};
+    const Span in_o[3] = {o_in_x ? none : sx, o_in_r ? none : sr, sg}, in_y[3] = {y_in_x ? none : sx, y_in_r ? none : sr, sg};
+    const Span in_q[3] = {sx, sr, sg}, out4[4] = {so, sy, sc, ss};
+    if (!no_overlap(out4, 4, nullptr, 0, "rmsnorm") || !no_overlap(&so, 1, in_o, 3, "rmsnorm") ||
+        !no_overlap(&sy, 1, in_y, 3, "rmsnorm") || !no_overlap(out4 + 2, 2, in_q, 3, "rmsnorm"))
+        return 1;
+    OnDevice0 dev;
+    if (!ensure_init()) return 1;
+    ApusNormArgs a{};
+    a.x = x; a.res = res; a.gamma = gamma; a.res_out = res_out; a.y = y; a.codes = codes; a.scales = scales;
+    a.M = M; a.K = K; a.ldx = ldx; a.eps = eps;
+    a.x_bf16 = xb; a.y_bf16 = yb; a.gamma_bf16 = (flags & APUS_HIP_W_BF16) != 0;
+    a.round_y = (flags & APUS_HIP_R_OUT) != 0; a.q_i8 = i8;
+    return launched(apus_launch_rmsnorm(&a, dev_stream()), "rmsnorm") ? 0 : 1;
+}
+
+int apus_hip_route_dev(const ApusHipRoute *cfg, const float *logits, const float *bias, int s, int E, int32_t *idx,
+                       float *wgt, float *scores) {
+    static_assert(APUS_HIP_SCORE_SQRTSOFTPLUS == APUS_SCORE_SQRTSOFTPLUS && APUS_HIP_SCORE_SIGMOID == APUS_SCORE_SIGMOID &&
+                  APUS_HIP_SCORE_SOFTMAX == APUS_SCORE_SOFTMAX, "score kinds");
+    if (!cfg || cfg->score < 0 || cfg->score > APUS_HIP_SCORE_SOFTMAX || (cfg->renorm & ~1) ||
+        !(cfg->route_scale - cfg->route_scale == 0.0f)) {
+        set_err("route: bad score kind, renorm (0 or 1) or scale");
+        return 1;
+    }
+    if (s < 0 || s > ROWS_LIMIT || E <= 0 || E > 1024 || cfg->topk <= 0 || cfg->topk > 16) {
+        set_err("route: unsupported shape s=%d E=%d topk=%d (E <= 1024, topk <= 16)", s, E, cfg->topk);
+        return 1;
+    }
+    if (cfg->n_group <= 0 || cfg->n_group > 64 || E % cfg->n_group || cfg->topk_group <= 0 ||
+        cfg->topk_group > cfg->n_group || cfg->group_top < 1 || cfg->group_top > 2 ||
+        cfg->topk > E / cfg->n_group * cfg->topk_group) {
+        set_err("route: %d groups of E=%d, %d kept by %d, cannot hold topk=%d (n_group <= 64 divides E, group_top 1 or 2)",
+                cfg->n_group, E, cfg->topk_group, cfg->group_top, cfg->topk);
+        return 1;
+    }
+    if (!logits || !idx || !wgt || !aligned(logits, 4) || !aligned(bias, 4) || !aligned(idx, 4) || !aligned(wgt, 4) ||
+        !aligned(scores, 4)) {
+        set_err("route: null or misaligned array");
+        return 1;
+    }
+    if (s == 0) return 0;
+    const size_t n = (size_t)s * E * 4, k = (size_t)s * cfg->topk * 4;
+    const Span in[2] = {{logits, n}, {bias, (size_t)E * 4}}, out[3] = {{idx, k}, {wgt, k}, {scores, n}};
+    if (!no_overlap(out, 3, in, 2, "route")) return 1;
+    OnDevice0 dev;
+    if (!ensure_init()) return 1;
+    ApusRouteArgs a{logits, bias, idx, wgt, scores, s, E, cfg->score, cfg->topk, cfg->n_group, cfg->topk_group,
+                    cfg->group_top, cfg->renorm, cfg->route_scale};
+    return launched(apus_launch_route(&a, dev_stream()), "route") ? 0 : 1;
+}
+
+int apus_hip_i8_quant_dev(const void *x, int M, int K, int flags, int8_t *codes, float *scales) {
+    const bool xb = flags & APUS_HIP_X_BF16;
+    if (flags & ~APUS_HIP_X_BF16) { set_err("i8_quant: unknown flags %#x", flags); return 1; }
+    if (M < 0 || K <= 0 || M > ROWS_LIMIT || K > ROWS_LIMIT) { set_err("i8_quant: unsupported shape M=%d K=%d", M, K); return 1; }
+    if (!x || !codes || !scales || !aligned(x, xb ? 2 : 4) || !aligned(scales, 4)) {
+        set_err("i8_quant: null or misaligned array");
+        return 1;
+    }
+    if (M == 0) return 0;
+    const size_t n = (size_t)M * K;
+    const Span in{x, n * (xb ? 2 : 4)}, out[2] = {{codes, n}, {scales, (size_t)M * 4}};
+    if (!no_overlap(out, 2, &in, 1, "i8_quant")) return 1;
+    OnDevice0 dev;
+    if (!ensure_init()) return 1;
+    return launched(apus_launch_i8_quant(x, xb, M, K, codes, scales, dev_stream()), "i8_quant") ? 0 : 1;
+}
+
+int apus_hip_i8_gemm_dev(const int8_t *w, const float *wscale, const int8_t *acodes, const float *ascale, void *out,
+                         int M, int O, int K, int flags) {
+    if (!i8_args_ok(w, wscale, acodes, out, M, O, K, flags, APUS_HIP_R_OUT | APUS_HIP_Y_BF16, "i8_gemm")) return 1;
+    if (!ascale || !aligned(ascale, 4)) { set_err("i8_gemm: null or misaligned array"); return 1; }
+    if (M == 0) return 0;
+    const Span o{out, (size_t)M * O * (flags & APUS_HIP_Y_BF16 ? 2 : 4)};
+    const Span in[4] = {{w, (size_t)O * K}, {wscale, (size_t)O * 4}, {acodes, (size_t)M * K}, {ascale, (size_t)M * 4}};
+    if (!no_overlap(&o, 1, in, 4, "i8_gemm")) return 1;
+    OnDevice0 dev;
+    if (!ensure_init()) return 1;
+    ApusI8Args a{w, acodes, wscale, ascale, out, M, O, K, (flags & APUS_HIP_Y_BF16) != 0, (flags & APUS_HIP_R_OUT) != 0};
+    return launched(apus_launch_i8_gemm(&a, dev_stream()), "i8_gemm") ? 0 : 1;
+}
+
+size_t apus_hip_i8_linear_workspace(int M, int K) {
+    return M <= 0 || K <= 0 ? 0 : align256((size_t)M * K) + align256((size_t)M * 4);
+}
+
+int apus_hip_i8_linear_dev(const int8_t *w, const float *wscale, const void *x, void *out, int M, int K, int O,
+                           int flags, void *workspace) {
+    if (!i8_args_ok(w, wscale, x, out, M, O, K, flags, APUS_HIP_R_OUT | APUS_HIP_Y_BF16 | APUS_HIP_X_BF16, "i8_linear"))
+        return 1;
+    if (M == 0) return 0;
+    if (!workspace || !aligned(workspace, 16)) { set_err("i8_linear: a 16-byte aligned workspace is required"); return 1; }
+    const int xb = (flags & APUS_HIP_X_BF16) != 0, yb = (flags & APUS_HIP_Y_BF16) != 0;
+    const Span o[2] = {{out, (size_t)M * O * (yb ? 2 : 4)}, {workspace, apus_hip_i8_linear_workspace(M, K)}};
+    const Span in[3] = {{w, (size_t)O * K}, {wscale, (size_t)O * 4}, {x, (size_t)M * K * (xb ? 2 : 4)}};
+    if (!no_overlap(o, 2, in, 3, "i8_linear")) return 1;
+    OnDevice0 dev;
+    if (!ensure_init()) return 1;
+    int8_t *c = (int8_t *)workspace;
+    float *s = (float *)(c + align256((size_t)M * K));
+    if (!launched(apus_launch_i8_quant(x, xb, M, K, c, s, dev_stream()), "i8_quant")) return 1;
+    ApusI8Args a{w, c, wscale, s, out, M, O, K, yb, (flags & APUS_HIP_R_OUT) != 0};
+    return launched(apus_launch_i8_gemm(&a, dev_stream()), "i8_gemm") ? 0 : 1;
+}
+
 /* ------------------------------------------------------------- the store */
 
 ApusHipStore *apus_hip_store_create(int n_layers, int E, int dim, int inter, char *err,

@@ -311,4 +311,41 @@ hipError_t apus_launch_swiglu(const float *g, const float *u, size_t n, float li
 hipError_t apus_launch_store_fill(uint8_t *base, size_t stride, int E, int O, int K, int what,
                                   int tiled, uint64_t seed, uint64_t sid0, hipStream_t st);
 
+/* RMS norm of rows with the residual's addition and 8-bit output
+ * (apus_hip_rmsnorm_dev); pointers that are NULL are not read or written */
+typedef struct {
+    const void *x, *res, *gamma;
+    void *res_out, *y;
+    uint8_t *codes;
+    float *scales;
+    int M, K, ldx;
+    float eps;
+    int x_bf16, y_bf16, gamma_bf16, round_y, q_i8;
+} ApusNormArgs;
+hipError_t apus_launch_rmsnorm(const ApusNormArgs *a, hipStream_t st);
+
+/* integer codes [M, K] and scales [M] of rows */
+hipError_t apus_launch_i8_quant(const void *x, int x_bf16, int M, int K, int8_t *codes, float *scales,
+                                hipStream_t st);
+
+/* expert choice from logits (apus_hip_route_dev) */
+enum { APUS_SCORE_SQRTSOFTPLUS = 0, APUS_SCORE_SIGMOID = 1, APUS_SCORE_SOFTMAX = 2 };
+typedef struct {
+    const float *logits, *bias;
+    int32_t *idx;
+    float *wgt, *scores;
+    int s, E, score, topk, groups, keep, group_top, renorm;
+    float route_scale;
+} ApusRouteArgs;
+hipError_t apus_launch_route(const ApusRouteArgs *a, hipStream_t st);
+
+/* integer product (apus_hip_i8_gemm_dev) */
+typedef struct {
+    const int8_t *w, *a;          /* [O, K], [M, K] */
+    const float *ws, *as;         /* [O], [M] */
+    void *out;                    /* [M, O] */
+    int M, O, K, y_bf16, round_out;
+} ApusI8Args;
+hipError_t apus_launch_i8_gemm(const ApusI8Args *a, hipStream_t st);
+
 #endif /* APUS_INTERNAL_H */

@@ -66,6 +66,10 @@ typedef struct {
 #define APUS_HIP_R_IN   1      /* BF16-round the input elements */
 #define APUS_HIP_R_OUT  2      /* BF16-round the output */
 #define APUS_HIP_W_BF16 4      /* w holds BF16 bits (uint16), not FP32 */
+/* further flags of the norm and integer entry points */
+#define APUS_HIP_X_BF16 8      /* activations (x, res, res_out) hold BF16 bits */
+#define APUS_HIP_Y_BF16 16     /* the output is stored as BF16 bits */
+#define APUS_HIP_Q_I8   32     /* codes are integers with one scale a row */
 
 #ifndef APUS_FP4_H
 /* c/fp4.h:184-188 — one entry of a grouped same-(O,K) MXFP4 GEMM */
@@ -357,6 +361,73 @@ int      apus_hip_moe_routed_h(const ApusHipStore *st, int s, int topk, const vo
  * flags as apus_hip_f32_linear. */
 int      apus_hip_wlinear_dev(const void *w, const float *x, float *out, int M, int K,
                               int O, int flags);
+
+/* ---- norm, routing and integer products (device pointers, asynchronous) ----
+ * No counterpart in the reference's boundary. Zero rows or tokens are a call
+ * with nothing to do; a refused call launches nothing. fp32 arrays are 4-byte,
+ * BF16 arrays 2-byte aligned; an output may overlap no other array unless said.
+ */
+/* RMS norm of M rows of K elements, the residual's addition before it and the
+ * codes of a quantised product behind it:
+ *   r = x + res (res NULL: r = x), rounded to BF16 with X_BF16, to res_out if given
+ *   y = r * gamma / sqrt(mean(r^2) + eps), evaluated in 64 bits, rounded to fp32
+ *       (and to BF16 with R_OUT or Y_BF16), to y if given
+ *   codes [M, K] and scales of bf16(y), if given:
+ *       E4M3 and scales [M, K/128] as apus_hip_act_quant_dev (K % 128 == 0), or
+ *       with Q_I8 integers and scales [M] as apus_hip_i8_quant_dev
+ * x has row stride ldx >= K elements; res, res_out, y and codes are [M, K].
+ * gamma [K] is fp32 (BF16 with W_BF16) and finite; eps > 0. res_out may be res,
+ * or x where ldx == K; y may be x (ldx == K) or res where their types are the
+ * same. Rows with a non-finite r: y as the formula gives it, codes 0 and scales
+ * +inf (E4M3) or NaN (integers), so that products return NaN for that row only. */
+int apus_hip_rmsnorm_dev(const void *x, int ldx, const void *res, void *res_out,
+                         const void *gamma, int M, int K, float eps, int flags, void *y,
+                         uint8_t *codes, float *scales);
+
+/* Expert choice for s tokens from router logits [s, E] (apus_hip_wlinear_dev of
+ * the gate's weight gives them): idx [s, topk] and wgt [s, topk] as
+ * apus_hip_moe_routed_dev takes them.
+ *   p = score(logit); sel = p + bias (bias [E] or NULL)
+ *   n_group > 1: the experts are n_group runs of E / n_group; a group's score is
+ *     the sum of its group_top (1 or 2) largest sel; only the topk_group best
+ *     groups take part
+ *   the topk largest sel, in descending order; wgt = p (over the sum of the chosen
+ *     p with renorm) * route_scale
+ * scores [s, E], if given, receives p of every expert. p, sel and the weights are
+ * evaluated in 64 bits, so the choice does not depend on how an exponential was
+ * rounded; ties (experts or groups) go to the lowest index. Experts whose logit
+ * or bias is -inf or NaN are masked: chosen last, lowest index first, with weight
+ * 0 (and left out of a group's sum); their p is 0 where the logit masks them. A
+ * weight sum of 0 gives zeros. +inf is read as the largest fp32.
+ * E <= 1024, topk <= 16, n_group <= 64, topk <= topk_group * (E / n_group). */
+#define APUS_HIP_SCORE_SQRTSOFTPLUS 0   /* sqrt(log(1 + exp(logit))) */
+#define APUS_HIP_SCORE_SIGMOID      1
+#define APUS_HIP_SCORE_SOFTMAX      2   /* over all E logits */
+typedef struct {
+    int score, topk;
+    int n_group, topk_group, group_top;   /* 1, 1, 1: no groups */
+    int renorm;
+    float route_scale;
+} ApusHipRoute;
+int apus_hip_route_dev(const ApusHipRoute *cfg, const float *logits, const float *bias, int s,
+                       int E, int32_t *idx, float *wgt, float *scores);
+
+/* Integer codes [M, K] and scales [M] of the rows of x [M, K] (fp32, or BF16
+ * with X_BF16; activations, or a weight's rows = its channels): b = bf16(x), a =
+ * max(max |b|, 2^-100), scale = fp32(a / 127), code = rint(fp32(b * fp32(127 /
+ * a))), -127..127. A row with a non-finite element: codes 0, scale NaN. */
+int apus_hip_i8_quant_dev(const void *x, int M, int K, int flags, int8_t *codes, float *scales);
+/* Product of integer codes: out[m, o] = (fp32(sum_k a[m, k] w[o, k]) * ascale[m]) *
+ * wscale[o], the sum exact. w [O, K], acodes [M, K], out [M, O] fp32 (BF16-rounded
+ * with R_OUT) or BF16 (Y_BF16). K % 4 == 0, K <= 131068, codes 4-byte aligned;
+ * K % 16 == 0 and 16-byte alignment take the fast schedules, bit for bit alike. */
+int apus_hip_i8_gemm_dev(const int8_t *w, const float *wscale, const int8_t *acodes,
+                         const float *ascale, void *out, int M, int O, int K, int flags);
+/* Linear = i8_quant of x [M, K] (X_BF16: BF16) + product, with a caller workspace
+ * of apus_hip_i8_linear_workspace(M, K) bytes (16-byte aligned); flags of both. */
+size_t apus_hip_i8_linear_workspace(int M, int K);
+int apus_hip_i8_linear_dev(const int8_t *w, const float *wscale, const void *x, void *out, int M,
+                           int K, int O, int flags, void *workspace);
 
 /* ---- apus model containers: routed-expert slabs on disk -> the store ----
  *
