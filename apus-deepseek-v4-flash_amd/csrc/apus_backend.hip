@@ -1496,7 +1496,8 @@ int apus_hip_i8_gemm_dev(const int8_t *w, const float *wscale, const int8_t *aco
     if (!no_overlap(&o, 1, in, 4, "i8_gemm")) return 1;
     OnDevice0 dev;
     if (!ensure_init()) return 1;
-    ApusI8Args a{w, acodes, wscale, ascale, out, M, O, K, (flags & APUS_HIP_Y_BF16) != 0, (flags & APUS_HIP_R_OUT) != 0};
+    ApusI8Args a{w, acodes, wscale, ascale, nullptr, out, M, O, K, (flags & APUS_HIP_Y_BF16) != 0, (flags & APUS_HIP_R_OUT) != 0,
+                 0};
     return launched(apus_launch_i8_gemm(&a, dev_stream()), "i8_gemm") ? 0 : 1;
 }
 
@@ -1518,8 +1519,13 @@ int apus_hip_i8_linear_dev(const int8_t *w, const float *wscale, const void *x, 
     if (!ensure_init()) return 1;
     int8_t *c = (int8_t *)workspace;
     float *s = (float *)(c + align256((size_t)M * K));
-    if (!launched(apus_launch_i8_quant(x, xb, M, K, c, s, dev_stream()), "i8_quant")) return 1;
-    ApusI8Args a{w, c, wscale, s, out, M, O, K, yb, (flags & APUS_HIP_R_OUT) != 0};
+    ApusI8Args a{w, nullptr, wscale, nullptr, x, out, M, O, K, yb, (flags & APUS_HIP_R_OUT) != 0, xb};
+    if (!apus_i8_fused_ok(&a)) {
+        if (!launched(apus_launch_i8_quant(x, xb, M, K, c, s, dev_stream()), "i8_quant")) return 1;
+        a.x = nullptr;
+        a.a = c;
+        a.as = s;
+    }
     return launched(apus_launch_i8_gemm(&a, dev_stream()), "i8_gemm") ? 0 : 1;
 }
 

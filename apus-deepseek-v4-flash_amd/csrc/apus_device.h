@@ -237,4 +237,22 @@ __device__ __forceinline__ float apus_route_weight(const float *chp, int topk, i
     return chp[j] / sum * route_scale;
 }
 
+/* Scale and reciprocal of a row's integer codes from its largest |b|, at least
+ * 2^-100 (127 / a and a / 127 stay normal fp32); not finite: NaN and 0. */
+__device__ __forceinline__ void apus_i8_scale(float amax, float &scale, float &inv) {
+    if (!(amax < __builtin_inff())) {
+        scale = __builtin_nanf("");
+        inv = 0.0f;
+        return;
+    }
+    const double a = fmax((double)amax, 0x1p-100);
+    scale = (float)(a / 127.0);
+    inv = (float)(127.0 / a);
+}
+/* |b| <= a, so |b inv| is 127 at most after rounding; NaN (a non-finite row) -> 0 */
+__device__ __forceinline__ int apus_i8_code(float b, float inv) {
+    const float q = __builtin_rintf(b * inv);
+    return (int)(q > 127.0f ? 127.0f : q < -127.0f ? -127.0f : q == q ? q : 0.0f);
+}
+
 #endif /* APUS_DEVICE_H */

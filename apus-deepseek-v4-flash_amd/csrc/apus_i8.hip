@@ -9,6 +9,8 @@
 
 #include <algorithm>
 
+typedef int apus_v4i __attribute__((ext_vector_type(4)));
+
 namespace {
 
 template <bool YB>
@@ -19,6 +21,49 @@ __device__ __forceinline__ void i8_store(void *out, size_t i, int acc, float sa,
     } else {
         apus_gst<float>((float *)out + i, round_out ? apus_bf16_rne(v) : v);
     }
+}
+
+/* the bits of four BF16 values */
+__device__ __forceinline__ uint64_t bf16x4(const float (&v)[4]) {
+    return (uint64_t)apus_bf16_bits(v[0]) | (uint64_t)apus_bf16_bits(v[1]) << 16 | (uint64_t)apus_bf16_bits(v[2]) << 32 |
+           (uint64_t)apus_bf16_bits(v[3]) << 48;
+}
+
+/* outputs (m, o .. o + 3): one store where the row's pieces are aligned for it */
+template <bool YB>
+__device__ __forceinline__ void i8_store4(const ApusI8Args &a, int m, int o, apus_v4i acc) {
+    constexpr int E = YB ? 2 : 4;
+    const float sa = a.as[m];
+    const size_t i = (size_t)m * a.O + o;
+    if (((a.O * (size_t)E | (uintptr_t)a.out) & (4 * E - 1)) == 0 && ((uintptr_t)a.ws & 15) == 0 && o < a.O) {
+        const apus_v4f sw = *reinterpret_cast<const apus_v4f *>(a.ws + o);
+        float v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            v[k] = ((float)acc[k] * sa) * sw[k];
+            if (YB || a.round_out) v[k] = apus_bf16_rne(v[k]);
+        }
+        if constexpr (YB)
+            apus_gst<uint64_t>((uint16_t *)a.out + i, bf16x4(v));
+        else
+            apus_gst<apus_v4f>((float *)a.out + i, apus_v4f{v[0], v[1], v[2], v[3]});
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        if (o + k < a.O) i8_store<YB>(a.out, i + k, acc[k], sa, a.ws[o + k], a.round_out);
+}
+
+/* tile of workgroup b: each XCD (workgroups are dealt to the 8 XCDs round robin)
+ * takes a contiguous band of tiles, ordered in groups of up to 8 row blocks by
+ * every column block, so that the tiles running together on an XCD share both
+ * operands in its L2 */
+__device__ __forceinline__ void apus_i8_tile(unsigned b, int mt, int nt, int &mb, int &nb) {
+    const unsigned tiles = (unsigned)mt * nt, per = tiles >> 3, rem = tiles & 7, x = b & 7;
+    const unsigned t = x * per + min(x, rem) + (b >> 3);
+    const unsigned grp = t / (8u * nt), g0 = grp * 8, gm = min(8u, mt - g0), in = t - grp * 8 * nt;
+    mb = g0 + in % gm;
+    nb = in / gm;
 }
 
 }  // namespace
@@ -60,8 +105,491 @@ __global__ __launch_bounds__(256) void apus_i8_any_kernel(ApusI8Args a) {
     }
 }
 
+/*
+ * Block schedule: a workgroup of WM x WN waves owns BM activation rows x BN
+ * weight rows. Both operands travel global -> LDS in steps of 128 bytes of K (8
+ * whole 128-byte rows a load, NST stages), chunk c of row i in slot c ^ (i / 2 %
+ * 8): the 16 rows that a quarter of a wave reads lie in 64 different banks. From
+ * there fragments go into a second set of registers one matrix instruction's
+ * depth ahead, so that a stage is free for its next load at the barrier behind
+ * its last read. The weights are the first operand, so a lane has four neighbouring
+ * outputs of one row. Rows past M or O repeat the last one; past K the activations are
+ * zeroed in LDS (0 times whatever the clamped weight bytes are).
+ */
+template <int BM_, int BN_, int WM_, int WN_, int NST_>
+struct ApusI8Blk {
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NST = NST_, NW = WM * WN;
+    static constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
+    static constexpr int LX = BM / 8, LT = (BM + BN) / 8, LPW = (LT + NW - 1) / NW;  /* loads: activations, all, a wave's */
+    static constexpr int STB = (BM + BN) * 128, LDS = NST * STB + (BM + BN) * 4;  /* stages; scales */
+    static_assert(BM % (WM * 16) == 0 && BN % (WN * 16) == 0 && (BM + BN) % 64 == 0 && LDS <= 160 * 1024, "block shape");
+};
+
+template <class B, bool YB>
+__global__ __launch_bounds__(64 * B::NW) void apus_i8_block_kernel(ApusI8Args a) {
+    constexpr int TM = B::TM, TN = B::TN, NST = B::NST;
+    extern __shared__ __align__(16) uint8_t lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, g = lane >> 4, wm = wave / B::WN, wn = wave % B::WN;
+    const int mt = (a.M + B::BM - 1) / B::BM, nt = (a.O + B::BN - 1) / B::BN;
+    int mb, nb;
+    apus_i8_tile(blockIdx.x, mt, nt, mb, nb);
+    const int m0 = mb * B::BM, n0 = nb * B::BN, K = a.K, nq = (K + 127) >> 7, tail = K & 127;
+    const unsigned lbase = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)lds);
+    /* a wave's loads (the last ones again where they do not divide evenly): a
+     * uniform base and 32-bit lane offsets; the last step's chunks past K read the
+     * row's last chunk */
+    const uint8_t *xb = (const uint8_t *)a.a + (size_t)m0 * K, *wb = (const uint8_t *)a.w + (size_t)n0 * K;
+    unsigned off[B::LPW];
+    int chunk[B::LPW];
+    auto load_of = [&](int u) { return min(wave * B::LPW + u, B::LT - 1); };
+#pragma unroll
+    for (int u = 0; u < B::LPW; ++u) {
+        const int ii = load_of(u), i = 8 * (ii < B::LX ? ii : ii - B::LX) + (lane >> 3);
+        chunk[u] = (lane & 7) ^ ((i >> 1) & 7);
+        off[u] = (unsigned)min(i, (ii < B::LX ? a.M - m0 : a.O - n0) - 1) * (unsigned)K + chunk[u] * 16;
+    }
+    auto issue = [&](int q, int slot) {
+        const bool last = tail && q == nq - 1;
+#pragma unroll
+        for (int u = 0; u < B::LPW; ++u) {
+            const int ii = load_of(u);
+            unsigned o = off[u];
+            if (last) o -= max(0, chunk[u] * 16 - (tail - 16));
+            asm("" : "+v"(o));                                   /* 32 bits beside the uniform base */
+            apus_g2lds16((ii < B::LX ? xb : wb) + (size_t)q * 128 + o, lbase + slot * B::STB + ii * 1024);
+        }
+    };
+    /* the activation chunks past K that this wave loaded, once they are in LDS */
+    auto zero_tail = [&](int slot) {
+#pragma unroll
+        for (int u = 0; u < B::LPW; ++u)
+            if (load_of(u) < B::LX && chunk[u] * 16 >= tail)
+                *reinterpret_cast<apus_v4i *>(lds + slot * B::STB + load_of(u) * 1024 + lane * 16) = apus_v4i{0, 0, 0, 0};
+    };
+    struct Frag { apus_v4i w[TN], x[TM]; };
+    const int sw = (r >> 1) & 7;
+    auto read = [&](Frag &f, int slot, int s) {
+        const uint8_t *stg = lds + slot * B::STB;
+        const int c = ((4 * s + g) ^ sw) << 4;
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+            f.w[i] = *reinterpret_cast<const apus_v4i *>(stg + (B::BM + (wn * TN + i) * 16 + r) * 128 + c);
+#pragma unroll
+        for (int t = 0; t < TM; ++t)
+            f.x[t] = *reinterpret_cast<const apus_v4i *>(stg + ((wm * TM + t) * 16 + r) * 128 + c);
+    };
+    apus_v4i acc[TN][TM];
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int t = 0; t < TM; ++t) acc[i][t] = apus_v4i{0, 0, 0, 0};
+    auto mul = [&](const Frag &f) {
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+#pragma unroll
+            for (int t = 0; t < TM; ++t)
+                acc[i][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f.w[i], f.x[t], acc[i][t], 0, 0, 0);
+    };
+    /* the fragment reads spread among the matrix instructions */
+    auto weave = [&]() {
+        constexpr int NR = TM + TN, NM = TM * TN, PER = (NR + NM - 1) / NM;
+#pragma unroll
+        for (int i = 0; i < NM; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        }
+    };
+    /* scales of the block's rows, then of its columns, to LDS */
+    for (int i = wave; i < (B::BM + B::BN) / 64; i += B::NW) {     /* older than every stage: counted with the first */
+        const int k = 64 * i + lane;
+        apus_g2lds4(k < B::BM ? a.as + min(m0 + k, a.M - 1) : a.ws + min(n0 + k - B::BM, a.O - 1),
+                    lbase + NST * B::STB + i * 256);
+    }
+    const int pre = min(nq, NST);
+    for (int q = 0; q < pre; ++q) issue(q, q);
+    /* stage q complete: only the stages behind it may be in flight */
+    auto arrive = [&](int q, int slot, int issued) {
+        const int behind = issued - 1 - q;
+        if (NST > 3 && behind >= 3)      apus_wait_vm<3 * B::LPW>();
+        else if (NST > 2 && behind >= 2) apus_wait_vm<2 * B::LPW>();
+        else if (behind >= 1)            apus_wait_vm<B::LPW>();
+        else                             apus_wait_vm<0>();
+        if (tail && q == nq - 1) zero_tail(slot);
+        apus_lds_barrier();
+    };
+    arrive(0, 0, pre);
+    Frag fr[2];
+    read(fr[0], 0, 0);
+    int slot = 0;
+    for (int q = 0; q < nq; ++q) {
+        const int nxt = slot + 1 == NST ? 0 : slot + 1;
+        read(fr[1], slot, 1);
+        mul(fr[0]);
+        weave();
+        __builtin_amdgcn_sched_barrier(0);
+        if (q + 1 < nq) {
+            arrive(q + 1, nxt, min(nq, q + NST));
+            if (q + NST < nq) issue(q + NST, slot);
+            __builtin_amdgcn_sched_barrier(0);
+            read(fr[0], nxt, 0);
+        }
+        mul(fr[1]);
+        weave();
+        __builtin_amdgcn_sched_barrier(0);
+        slot = nxt;
+    }
+    /* Outputs: 16 rows at a time through a wave's own LDS, so that a store writes whole
+     * lines. A lane holds row r, columns 4 g .. 4 g + 3 of each tile. */
+    constexpr int E = YB ? 2 : 4, CW = TN * 16, PITCH = CW * E + 16;
+    constexpr int LR = CW * E / 16;                             /* 16-byte pieces of a row */
+    static_assert(B::NW * 16 * PITCH <= NST * B::STB && 64 % LR == 0, "output staging");
+    __syncthreads();
+    const float *las = reinterpret_cast<const float *>(lds + NST * B::STB) + wm * TM * 16;
+    const float *lws = reinterpret_cast<const float *>(lds + NST * B::STB) + B::BM + wn * CW;
+    uint8_t *ob = lds + wave * (16 * PITCH);
+    apus_v4f sw4[TN];
+#pragma unroll
+    for (int i = 0; i < TN; ++i) sw4[i] = *reinterpret_cast<const apus_v4f *>(lws + i * 16 + 4 * g);
+    const int col = n0 + wn * CW + lane % LR * (16 / E);
+    const bool whole = ((a.O * (size_t)E | (uintptr_t)a.out) & 15) == 0 && col + 16 / E <= a.O;
+#pragma unroll
+    for (int t = 0; t < TM; ++t) {
+        const float sa = las[t * 16 + r];
+#pragma unroll
+        for (int i = 0; i < TN; ++i) {
+            float v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                v[k] = ((float)acc[i][t][k] * sa) * sw4[i][k];
+                if (YB || a.round_out) v[k] = apus_bf16_rne(v[k]);
+            }
+            uint8_t *d = ob + r * PITCH + (i * 16 + 4 * g) * E;
+            if constexpr (YB) *reinterpret_cast<uint64_t *>(d) = bf16x4(v);
+            else              *reinterpret_cast<apus_v4f *>(d) = apus_v4f{v[0], v[1], v[2], v[3]};
+        }
+        asm volatile("" ::: "memory");                          /* a wave's LDS operations run in order */
+#pragma unroll
+        for (int p = 0; p < (16 * LR + 63) / 64; ++p) {
+            const int row = p * (64 / LR) + lane / LR, m = m0 + (wm * TM + t) * 16 + row;
+            if (row >= 16) break;
+            const apus_v4u v = *reinterpret_cast<const apus_v4u *>(ob + row * PITCH + lane % LR * 16);
+            uint8_t *d = (uint8_t *)a.out + ((size_t)m * a.O + col) * E;
+            if (m < a.M && whole) {
+                apus_gst<apus_v4u>(d, v);
+            } else if (m < a.M) {
+#pragma unroll
+                for (int k = 0; k < 16 / E; ++k)
+                    if (col + k < a.O) {
+                        if constexpr (YB) apus_gst<uint16_t>(d + 2 * k, (uint16_t)(v[k >> 1] >> (16 * (k & 1))));
+                        else              apus_gst<uint32_t>(d + 4 * k, v[k]);
+                    }
+            }
+        }
+        asm volatile("" ::: "memory");
+    }
+}
+
+template <class B>
+hipError_t apus_launch_i8_block(const ApusI8Args &a, hipStream_t st) {
+    auto go = [&](auto kernel) {
+        static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
+                                                           hipFuncAttributeMaxDynamicSharedMemorySize, B::LDS);
+        if (attr != hipSuccess) return attr;
+        const size_t tiles = ((size_t)a.M + B::BM - 1) / B::BM * (((size_t)a.O + B::BN - 1) / B::BN);
+        if (tiles > 0xffffffffu / (64 * B::NW)) return hipErrorInvalidValue;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(64 * B::NW), B::LDS, st, a);
+        return hipGetLastError();
+    };
+    return a.y_bf16 ? go(&apus_i8_block_kernel<B, true>) : go(&apus_i8_block_kernel<B, false>);
+}
+
+/*
+ * Narrow schedule, up to 64 rows: a workgroup owns 16 TN weight rows and all M
+ * activation rows (TM tiles of 16; HALF: at most 8 rows, half a tile's loads);
+ * its NW waves split K, each bringing both operands through a ring of its own in
+ * LDS, PD steps of 128 bytes deep: no barrier in the loop. The waves' integer sums
+ * meet in LDS.
+ */
+template <int TM, int TN, int NW, int PD, bool HALF, bool YB>
+__global__ __launch_bounds__(64 * NW) void apus_i8_narrow_kernel(ApusI8Args a) {
+    constexpr int LX = HALF ? 1 : 2 * TM, NL = LX + 2 * TN, SLOT = NL * 1024;
+    static_assert((PD - 1) * NL < 64 && PD >= 2 && PD <= 4, "vmcnt");
+    extern __shared__ __align__(16) uint8_t lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, g = lane >> 4, K = a.K, nq = (K + 127) >> 7, tail = K & 127;
+    /* the row blocks of one column block follow each other on its XCD */
+    const int mt = (a.M + 16 * TM - 1) / (16 * TM), mb = (blockIdx.x >> 3) % mt;
+    const int n0 = (int)(((blockIdx.x >> 3) / mt) * 8 + (blockIdx.x & 7)) * 16 * TN, m0 = mb * 16 * TM;
+    if (n0 >= a.O) return;
+    const int q0 = (int)((size_t)nq * wave / NW), q1 = (int)((size_t)nq * (wave + 1) / NW);
+    uint8_t *ring = lds + wave * PD * SLOT;
+    const unsigned rbase = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)ring);
+    const uint8_t *xb = (const uint8_t *)a.a + (size_t)m0 * K, *wb = (const uint8_t *)a.w + (size_t)n0 * K;
+    unsigned off[NL];
+    int chunk[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) chunk[h] = (lane & 7) ^ ((4 * h + (lane >> 4)) & 7);
+#pragma unroll
+    for (int u = 0; u < NL; ++u) {
+        const int j = u < LX ? u : u - LX, i = 8 * j + (lane >> 3);
+        off[u] = (unsigned)min(i, (u < LX ? a.M - m0 : a.O - n0) - 1) * (unsigned)K + chunk[j & 1] * 16;
+    }
+    auto issue = [&](int q, int slot) {
+        const bool last = tail && q == nq - 1;
+#pragma unroll
+        for (int u = 0; u < NL; ++u) {
+            unsigned o = off[u];
+            if (last) o -= max(0, chunk[(u < LX ? u : u - LX) & 1] * 16 - (tail - 16));
+            asm("" : "+v"(o));
+            apus_g2lds16((u < LX ? xb : wb) + (size_t)q * 128 + o, rbase + slot * SLOT + u * 1024);
+        }
+    };
+    apus_v4i acc[TN][TM];
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int t = 0; t < TM; ++t) acc[i][t] = apus_v4i{0, 0, 0, 0};
+#pragma unroll
+    for (int d = 0; d < PD; ++d)
+        if (q0 + d < q1) issue(q0 + d, d);
+    const int sw = (r >> 1) & 7;
+    int slot = 0;
+    for (int q = q0; q < q1; ++q) {
+        const int later = min(q1 - 1 - q, PD - 1);
+        if (PD > 3 && later >= 3)      apus_wait_vm<3 * NL>();
+        else if (PD > 2 && later >= 2) apus_wait_vm<2 * NL>();
+        else if (later >= 1)           apus_wait_vm<NL>();
+        else                           apus_wait_vm<0>();
+        uint8_t *stg = ring + slot * SLOT;
+        if (tail && q == nq - 1) {
+#pragma unroll
+            for (int u = 0; u < LX; ++u)
+                if (chunk[u & 1] * 16 >= tail)
+                    *reinterpret_cast<apus_v4i *>(stg + u * 1024 + lane * 16) = apus_v4i{0, 0, 0, 0};
+            asm volatile("" ::: "memory");
+        }
+        apus_v4i w[TN][2], x[TM][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int c = ((4 * h + g) ^ sw) << 4;
+#pragma unroll
+            for (int i = 0; i < TN; ++i)
+                w[i][h] = *reinterpret_cast<const apus_v4i *>(stg + LX * 1024 + (16 * i + r) * 128 + c);
+            /* HALF: rows 8..15 read rows 0..7 again; their columns are not stored */
+#pragma unroll
+            for (int t = 0; t < TM; ++t)
+                x[t][h] = *reinterpret_cast<const apus_v4i *>(stg + (HALF ? r & 7 : 16 * t + r) * 128 + (HALF ? ((4 * h + g) ^ ((r & 7) >> 1)) << 4 : c));
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      /* slot read before its refill */
+        if (q + PD < q1) issue(q + PD, slot);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < TN; ++i)
+#pragma unroll
+                for (int t = 0; t < TM; ++t)
+                    acc[i][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[i][h], x[t][h], acc[i][t], 0, 0, 0);
+        slot = slot + 1 == PD ? 0 : slot + 1;
+    }
+    /* lane: activation row 16 t + r, weight rows n0 + 16 i + 4 g + k */
+    apus_v4i *red = reinterpret_cast<apus_v4i *>(lds);
+    if constexpr (NW > 1) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+#pragma unroll
+            for (int t = 0; t < TM; ++t) red[(wave * TN * TM + i * TM + t) * 64 + lane] = acc[i][t];
+        __syncthreads();
+    }
+#pragma unroll
+    for (int u = 0; u < TN * TM; ++u) {
+        if (NW > 1 && u % NW != wave) continue;
+        const int i = u / TM, t = u % TM, m = m0 + 16 * t + r, o = n0 + 16 * i + 4 * g;
+        apus_v4i v = NW > 1 ? red[u * 64 + lane] : acc[i][t];
+#pragma unroll
+        for (int k = 1; k < NW; ++k) v += red[(k * TN * TM + u) * 64 + lane];
+        if (m < a.M) i8_store4<YB>(a, m, o, v);
+    }
+}
+
+template <int TM, int TN, int NW, int PD, bool HALF>
+hipError_t apus_launch_i8_narrow(const ApusI8Args &a, hipStream_t st) {
+    constexpr int ring = NW * PD * ((HALF ? 1 : 2 * TM) + 2 * TN) * 1024, sums = NW * TM * TN * 1024;
+    constexpr int lds = ring > sums ? ring : sums;
+    static_assert(lds <= 160 * 1024, "LDS");
+    auto go = [&](auto kernel) {
+        static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
+                                                           hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (attr != hipSuccess) return attr;
+        const size_t wgs = ((size_t)a.O + 128 * TN - 1) / (128 * TN) * 8 * (((size_t)a.M + 16 * TM - 1) / (16 * TM));
+        if (wgs > 0xffffffffu / (64 * NW)) return hipErrorInvalidValue;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)wgs), dim3(64 * NW), lds, st, a);
+        return hipGetLastError();
+    };
+    return a.y_bf16 ? go(&apus_i8_narrow_kernel<TM, TN, NW, PD, HALF, true>) : go(&apus_i8_narrow_kernel<TM, TN, NW, PD, HALF, false>);
+}
+
+/*
+ * One row: dot products on the vector units. A wave takes R weight rows, U chunks of
+ * 1 KB (16 bytes a lane) of each under way at once; sums over the lanes by a
+ * reduce-scatter. XS: the activations are codes (0), or an fp32 (1) or BF16 (2) row
+ * that every workgroup quantises for itself into LDS while its first weights come.
+ */
+template <int R, int U, int XS, bool YB>
+__global__ __launch_bounds__(256) void apus_i8_gemv_kernel(ApusI8Args a) {
+    extern __shared__ __align__(16) uint8_t lds[];               /* XS: the row's codes */
+    __shared__ unsigned lmax[4];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int K = a.K, nc = (K + 1023) >> 10, n0 = (blockIdx.x * 4 + wave) * R;
+    const uint8_t *wr[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) wr[i] = (const uint8_t *)a.w + (size_t)min(n0 + i, a.O - 1) * K;
+    apus_v4i w[U][R];
+    auto load_w = [&](int c0) {                                  /* past K: the row's last bytes again */
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+                w[u][i] = __builtin_bit_cast(apus_v4i, apus_ld16_stream(wr[i] + min((c0 + u) * 1024 + lane * 16, K - 16)));
+    };
+    load_w(0);
+    float sa;
+    if constexpr (XS != 0) {
+        __builtin_amdgcn_sched_barrier(0);                       /* the weights are under way first */
+        auto ldx = [&](int k, float (&v)[4]) {
+            if constexpr (XS == 1) {
+                const float4 f = apus_gld<float4>((const float *)a.x + k);
+                v[0] = apus_bf16_rne(f.x); v[1] = apus_bf16_rne(f.y); v[2] = apus_bf16_rne(f.z); v[3] = apus_bf16_rne(f.w);
+            } else {
+                const uint64_t f = apus_gld<uint64_t>((const uint16_t *)a.x + k);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = apus_u2f((uint32_t)(f >> (16 * j)) << 16);
+            }
+        };
+        unsigned top = 0;
+        for (int k = threadIdx.x * 4; k < K; k += 1024) {
+            float v[4];
+            ldx(k, v);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) top = max(top, apus_f2u(v[j]) & 0x7fffffffu);
+        }
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, o, 64));
+        if (lane == 0) lmax[wave] = top;
+        apus_lds_barrier();
+        float inv;
+        apus_i8_scale(apus_u2f(max(max(lmax[0], lmax[1]), max(lmax[2], lmax[3]))), sa, inv);
+        for (int k = threadIdx.x * 4; k < K; k += 1024) {
+            float v[4];
+            ldx(k, v);
+            unsigned c = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) c |= (unsigned)(apus_i8_code(v[j], inv) & 0xff) << (8 * j);
+            *reinterpret_cast<unsigned *>(lds + k) = c;
+        }
+        apus_lds_barrier();
+    } else {
+        sa = a.as[0];
+    }
+    int v[R] = {};
+    for (int c0 = 0; c0 < nc; c0 += U) {
+        if (c0) load_w(c0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k = (c0 + u) * 1024 + lane * 16, kk = min(k, K - 16);
+            apus_v4i x;
+            if constexpr (XS != 0) x = *reinterpret_cast<const apus_v4i *>(lds + kk);
+            else                   x = apus_gld<apus_v4i>(a.a + kk);
+            if (k >= K) x = apus_v4i{0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[i] = __builtin_amdgcn_sdot4(w[u][i][j], x[j], v[i], false);
+        }
+    }
+    /* reduce-scatter: lane l ends up with row l's sum, its low bits in reverse */
+#pragma unroll
+    for (int off = 1, n = R; off <= 32; off <<= 1, n = n > 1 ? n >> 1 : 1) {
+        const bool up = lane & off;
+        if (n == 1) {
+            v[0] += __shfl_xor(v[0], off, 64);
+            continue;
+        }
+#pragma unroll
+        for (int j = 0; j < n / 2; ++j) {
+            const int keep = up ? v[n / 2 + j] : v[j], send = up ? v[j] : v[n / 2 + j];
+            v[j] = keep + __shfl_xor(send, off, 64);
+        }
+    }
+    static_assert(R == 1 || R == 2 || R == 4, "rows of a wave");
+    const int o = n0 + (R == 4 ? (lane & 1) * 2 + (lane >> 1) : lane);
+    if (lane < R && o < a.O) i8_store<YB>(a.out, o, v[0], sa, a.ws[o], a.round_out);
+}
+
+template <int R, int U, int XS>
+hipError_t apus_launch_i8_gemv(const ApusI8Args &a, hipStream_t st) {
+    auto go = [&](auto kernel) {
+        const size_t wgs = ((size_t)a.O + 4 * R - 1) / (4 * R);
+        if (wgs > 0xffffffffu / 256) return hipErrorInvalidValue;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)wgs), dim3(256), XS ? (a.K + 15) & ~15 : 0, st, a);
+        return hipGetLastError();
+    };
+    return a.y_bf16 ? go(&apus_i8_gemv_kernel<R, U, XS, true>) : go(&apus_i8_gemv_kernel<R, U, XS, false>);
+}
+
+template <int XS>
+hipError_t apus_launch_i8_gemv_x(const ApusI8Args &a, hipStream_t st) {
+    return a.K > 2048 ? apus_launch_i8_gemv<1, 4, XS>(a, st) : a.K > 1024 ? apus_launch_i8_gemv<2, 2, XS>(a, st)
+                                                                          : apus_launch_i8_gemv<4, 1, XS>(a, st);
+}
+
+/* one row, fp32 or BF16 in: quantised inside the product's launch */
+bool apus_i8_fused_ok(const ApusI8Args *a) {
+    return a->M == 1 && a->K % 16 == 0 && a->K <= 32768 && (((uintptr_t)a->x | (uintptr_t)a->w) & 15) == 0;
+}
+
 hipError_t apus_launch_i8_gemm(const ApusI8Args *a, hipStream_t st) {
     if (a->M <= 0) return hipSuccess;
+    if (a->x) return a->x_bf16 ? apus_launch_i8_gemv_x<2>(*a, st) : apus_launch_i8_gemv_x<1>(*a, st);
+    if (a->K % 16 == 0 && (((uintptr_t)a->a | (uintptr_t)a->w) & 15) == 0) {
+        if (a->M == 1) return apus_launch_i8_gemv_x<0>(*a, st);
+        if (a->M <= 8)
+            return a->O <= 16384 ? apus_launch_i8_narrow<1, 1, 4, 4, true>(*a, st) : apus_launch_i8_narrow<1, 2, 2, 4, true>(*a, st);
+        /* More rows: the schedule whose modelled time is least, R (c steps + e) + t us:
+         * steps of 128 bytes of K, R rounds of the 256 CUs (where two workgroups fit a
+         * CU, the share of a round), c, e and t fitted to 73 measured shapes (rms 8 to 16
+         * % of each; the choice is 2-3 % behind the best of them in the geometric mean). */
+        static const struct {
+            hipError_t (*launch)(const ApusI8Args &, hipStream_t);
+            int bm, bn;
+            bool two;
+            float c, e, t;
+        } sched[] = {
+            {apus_launch_i8_narrow<1, 1, 4, 4, false>, 16, 16, true, 0.059f, 0.59f, 1.86f},
+            {apus_launch_i8_narrow<2, 2, 2, 4, false>, 32, 32, false, 0.140f, 0.72f, 2.13f},
+            {apus_launch_i8_narrow<4, 2, 4, 2, false>, 64, 32, false, 0.170f, 2.37f, 0.62f},
+            {apus_launch_i8_narrow<4, 4, 4, 2, false>, 64, 64, false, 0.243f, 3.99f, 0.63f},
+            {apus_launch_i8_block<ApusI8Blk<64, 64, 4, 2, 4>>, 64, 64, true, 0.306f, 0.58f, 2.95f},
+            {apus_launch_i8_block<ApusI8Blk<64, 128, 2, 4, 4>>, 64, 128, false, 0.439f, 2.72f, 0.95f},
+            {apus_launch_i8_block<ApusI8Blk<128, 128, 2, 4, 4>>, 128, 128, false, 0.574f, 4.38f, 0.53f},
+            {apus_launch_i8_block<ApusI8Blk<128, 128, 2, 4, 2>>, 128, 128, true, 0.697f, 1.84f, 2.53f},
+            {apus_launch_i8_block<ApusI8Blk<256, 256, 2, 4, 2>>, 256, 256, false, 1.391f, 13.74f, -2.19f},
+        };
+        const float steps = (float)((a->K + 127) / 128);
+        int best = 0;
+        float least = 0.0f;
+        for (int i = 0; i < (int)(sizeof sched / sizeof *sched); ++i) {
+            const size_t wgs = ((size_t)a->M + sched[i].bm - 1) / sched[i].bm * (((size_t)a->O + sched[i].bn - 1) / sched[i].bn);
+            const float r = sched[i].two ? std::max(1.0f, (float)wgs / 256.0f) : (float)((wgs + 255) / 256);
+            const float us = r * (sched[i].c * steps + sched[i].e) + sched[i].t;
+            if (i == 0 || us < least) {
+                best = i;
+                least = us;
+            }
+        }
+        return sched[best].launch(*a, st);
+    }
     const size_t tiles = ((size_t)a->M + 63) / 64 * (((size_t)a->O + 63) / 64);
     auto go = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)std::min(tiles, (size_t)1 << 20)), dim3(256), 0, st, *a);

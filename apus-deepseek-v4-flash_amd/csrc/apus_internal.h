@@ -343,9 +343,12 @@ hipError_t apus_launch_route(const ApusRouteArgs *a, hipStream_t st);
 typedef struct {
     const int8_t *w, *a;          /* [O, K], [M, K] */
     const float *ws, *as;         /* [O], [M] */
+    const void *x;                /* instead of a and as: an fp32 or BF16 row (apus_i8_fused_ok) */
     void *out;                    /* [M, O] */
-    int M, O, K, y_bf16, round_out;
+    int M, O, K, y_bf16, round_out, x_bf16;
 } ApusI8Args;
+/* whether the product takes a->x itself, without apus_launch_i8_quant before it */
+bool apus_i8_fused_ok(const ApusI8Args *a);
 hipError_t apus_launch_i8_gemm(const ApusI8Args *a, hipStream_t st);
 
 #endif /* APUS_INTERNAL_H */

@@ -27,8 +27,6 @@
 
 namespace {
 
-constexpr double I8_FLOOR = 0x1p-100;     /* 127 / a and a / 127 stay normal fp32 */
-
 template <bool BF>
 __device__ __forceinline__ float ld_elem(const void *p, size_t i) {
     if constexpr (BF) return apus_u2f((uint32_t)((const uint16_t *)p)[i] << 16);
@@ -38,24 +36,6 @@ template <bool BF>
 __device__ __forceinline__ void st_elem(void *p, size_t i, float v) {
     if constexpr (BF) ((uint16_t *)p)[i] = apus_bf16_bits(apus_bf16_rne(v));
     else              ((float *)p)[i] = v;
-}
-
-/* scale and reciprocal of integer codes from the row's largest |b|; a not
- * finite: NaN and 0 */
-__device__ __forceinline__ void i8_scale(float amax, float &scale, float &inv) {
-    if (!(amax < __builtin_inff())) {
-        scale = __builtin_nanf("");
-        inv = 0.0f;
-        return;
-    }
-    const double a = fmax((double)amax, I8_FLOOR);
-    scale = (float)(a / 127.0);
-    inv = (float)(127.0 / a);
-}
-/* |b| <= a, so |b inv| is 127 at most after rounding; NaN (a non-finite row) -> 0 */
-__device__ __forceinline__ int i8_code(float b, float inv) {
-    const float q = __builtin_rintf(b * inv);
-    return (int)(q > 127.0f ? 127.0f : q < -127.0f ? -127.0f : q == q ? q : 0.0f);
 }
 
 }  // namespace
@@ -107,8 +87,8 @@ __global__ __launch_bounds__(256) void apus_rmsnorm_any_kernel(ApusNormArgs a) {
             for (size_t k = tid; k < K; k += 256) norm(k);
         } else if (a.q_i8) {
             float scale, inv;
-            i8_scale(bad ? __builtin_inff() : apus_bf16_rne((float)(pm * v)), scale, inv);
-            for (size_t k = tid; k < K; k += 256) a.codes[ro + k] = (uint8_t)(int8_t)i8_code(norm(k), inv);
+            apus_i8_scale(bad ? __builtin_inff() : apus_bf16_rne((float)(pm * v)), scale, inv);
+            for (size_t k = tid; k < K; k += 256) a.codes[ro + k] = (uint8_t)(int8_t)apus_i8_code(norm(k), inv);
             if (tid == 0) a.scales[m] = scale;
         } else {
             const int nab = a.K >> 7;
@@ -159,9 +139,9 @@ __global__ __launch_bounds__(256) void apus_i8_quant_any_kernel(const void *__re
         if ((tid & 63) == 0) red[tid >> 6] = m;
         __syncthreads();
         float scale, inv;
-        i8_scale(apus_u2f(max(max(red[0], red[1]), max(red[2], red[3]))), scale, inv);
+        apus_i8_scale(apus_u2f(max(max(red[0], red[1]), max(red[2], red[3]))), scale, inv);
         for (int k = tid; k < K; k += 256)
-            codes[off + k] = (int8_t)i8_code(apus_bf16_rne(ld_elem<XB>(x, off + k)), inv);
+            codes[off + k] = (int8_t)apus_i8_code(apus_bf16_rne(ld_elem<XB>(x, off + k)), inv);
         if (tid == 0) scales[row] = scale;
         __syncthreads();                   /* red is free again */
     }
