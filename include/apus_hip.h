@@ -393,9 +393,9 @@ int apus_hip_rmsnorm_dev(const void *x, int ldx, const void *res, void *res_out,
  *     groups take part
  *   the topk largest sel, in descending order; wgt = p (over the sum of the chosen
  *     p with renorm) * route_scale
- * scores [s, E], if given, receives p of every expert. p, sel and the weights are
- * evaluated in 64 bits, so the choice does not depend on how an exponential was
- * rounded; ties (experts or groups) go to the lowest index. Experts whose logit
+ * The choice and the weights are those of 64-bit p and sel, so they do not depend on
+ * how an exponential was rounded; ties (experts or groups) go to the lowest index.
+ * scores [s, E], if given, receives p of every expert in fp32, within 2^-21. Experts whose logit
  * or bias is -inf or NaN are masked: chosen last, lowest index first, with weight
  * 0 (and left out of a group's sum); their p is 0 where the logit masks them. A
  * weight sum of 0 gives zeros. +inf is read as the largest fp32.
