@@ -55,12 +55,15 @@ __device__ __forceinline__ void i8_store4(const ApusI8Args &a, int m, int o, apu
 }
 
 /* tile of workgroup b: each XCD (workgroups are dealt to the 8 XCDs round robin)
- * takes a contiguous band of tiles, ordered in groups of up to 8 row blocks by
- * every column block, so that the tiles running together on an XCD share both
- * operands in its L2 */
+ * takes a contiguous band of tiles */
+__device__ __forceinline__ unsigned apus_i8_band(unsigned b, unsigned tiles) {
+    const unsigned per = tiles >> 3, rem = tiles & 7, x = b & 7;
+    return x * per + min(x, rem) + (b >> 3);
+}
+/* row and column block of a workgroup: in groups of up to 8 row blocks by every column
+ * block, so that the tiles running together on an XCD share both operands in its L2 */
 __device__ __forceinline__ void apus_i8_tile(unsigned b, int mt, int nt, int &mb, int &nb) {
-    const unsigned tiles = (unsigned)mt * nt, per = tiles >> 3, rem = tiles & 7, x = b & 7;
-    const unsigned t = x * per + min(x, rem) + (b >> 3);
+    const unsigned t = apus_i8_band(b, (unsigned)mt * nt);
     const unsigned grp = t / (8u * nt), g0 = grp * 8, gm = min(8u, mt - g0), in = t - grp * 8 * nt;
     mb = g0 + in % gm;
     nb = in / gm;
@@ -115,6 +118,14 @@ __global__ __launch_bounds__(256) void apus_i8_any_kernel(ApusI8Args a) {
  * its last read. The weights are the first operand, so a lane has four neighbouring
  * outputs of one row. Rows past M or O repeat the last one; past K the activations are
  * zeroed in LDS (0 times whatever the clamped weight bytes are).
+ * 4096 x 8192 x 4096, 256 x 256 tiles: 122-127 us, 2.2 POP/s (a large library product of
+ * these sizes 130); the matrix cores are busy 49 % of its cycles at 2.1 GHz (the rest
+ * follows the barrier: the stage's wait, the skew of 8 waves), the 64 MB of outputs go out
+ * in two bursts. 1000 x 4096 x 8192, 128 x 128 tiles four stages deep: 46 us, one wave of
+ * tiles whose operand stream L2 -> LDS runs at 14 TB/s, about what all tiles reach.
+ * Outputs straight from registers 191 us instead of 129 (stores of 8 bytes to 16 rows);
+ * 32x32x32 instructions 139 (fragments of half the depth); the wave's priority raised around
+ * the instructions 130, and 45.7 for 46.8 with 128 x 128 tiles: not kept.
  */
 template <int BM_, int BN_, int WM_, int WN_, int NST_>
 struct ApusI8Blk {
@@ -305,11 +316,13 @@ hipError_t apus_launch_i8_block(const ApusI8Args &a, hipStream_t st) {
 }
 
 /*
- * Narrow schedule, up to 64 rows: a workgroup owns 16 TN weight rows and all M
- * activation rows (TM tiles of 16; HALF: at most 8 rows, half a tile's loads);
+ * Narrow schedule, for some tens of rows: a workgroup owns 16 TN weight rows and 16 TM
+ * activation rows (HALF: at most 8 rows, half a tile's loads);
  * its NW waves split K, each bringing both operands through a ring of its own in
  * LDS, PD steps of 128 bytes deep: no barrier in the loop. The waves' integer sums
- * meet in LDS.
+ * meet in LDS. 8 rows, 4096 x 8192: 8.0 us (33.5 MB at 4.2 TB/s; 5 us of them at the rate of
+ * a long stream), the rest launch, ramp and the sums; up to 64 rows 12.4, where 256
+ * workgroups read 134 MB of activations from L2.
  */
 template <int TM, int TN, int NW, int PD, bool HALF, bool YB>
 __global__ __launch_bounds__(64 * NW) void apus_i8_narrow_kernel(ApusI8Args a) {
@@ -318,10 +331,9 @@ __global__ __launch_bounds__(64 * NW) void apus_i8_narrow_kernel(ApusI8Args a) {
     extern __shared__ __align__(16) uint8_t lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, g = lane >> 4, K = a.K, nq = (K + 127) >> 7, tail = K & 127;
-    /* the row blocks of one column block follow each other on its XCD */
-    const int mt = (a.M + 16 * TM - 1) / (16 * TM), mb = (blockIdx.x >> 3) % mt;
-    const int n0 = (int)(((blockIdx.x >> 3) / mt) * 8 + (blockIdx.x & 7)) * 16 * TN, m0 = mb * 16 * TM;
-    if (n0 >= a.O) return;
+    const int mt = (a.M + 16 * TM - 1) / (16 * TM), nt = (a.O + 16 * TN - 1) / (16 * TN);
+    const unsigned t0 = apus_i8_band(blockIdx.x, (unsigned)mt * nt);     /* the row blocks of a column block in turn */
+    const int n0 = (int)(t0 / mt) * 16 * TN, m0 = (int)(t0 % mt) * 16 * TM;
     const int q0 = (int)((size_t)nq * wave / NW), q1 = (int)((size_t)nq * (wave + 1) / NW);
     uint8_t *ring = lds + wave * PD * SLOT;
     const unsigned rbase = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)ring);
@@ -422,7 +434,7 @@ hipError_t apus_launch_i8_narrow(const ApusI8Args &a, hipStream_t st) {
         static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
                                                            hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (attr != hipSuccess) return attr;
-        const size_t wgs = ((size_t)a.O + 128 * TN - 1) / (128 * TN) * 8 * (((size_t)a.M + 16 * TM - 1) / (16 * TM));
+        const size_t wgs = ((size_t)a.O + 16 * TN - 1) / (16 * TN) * (((size_t)a.M + 16 * TM - 1) / (16 * TM));
         if (wgs > 0xffffffffu / (64 * NW)) return hipErrorInvalidValue;
         hipLaunchKernelGGL(kernel, dim3((unsigned)wgs), dim3(64 * NW), lds, st, a);
         return hipGetLastError();
@@ -538,6 +550,11 @@ hipError_t apus_launch_i8_gemv(const ApusI8Args &a, hipStream_t st) {
     return a.y_bf16 ? go(&apus_i8_gemv_kernel<R, U, XS, true>) : go(&apus_i8_gemv_kernel<R, U, XS, false>);
 }
 
+/* Rows and chunks a wave: about 4 KB of weights under way in each, from as many rows as
+ * that takes (us, 1 x 4 / 2 x 2 / 4 x 1: K 8192, 4096 channels 7.1 / 7.6 / 8.8; K 4096, 1024
+ * channels 2.8 / 3.4 / 4.5, 129280 74 / 75 / 79 (7.1 TB/s); K 2048, 4096 channels 3.8 / 3.4 /
+ * 3.7; K 1024, 32768 channels 12.5 / 8.0 / 7.0; more of a row or more rows at once are
+ * slower everywhere). Bound by HBM, or by the launch and one pass of latency. */
 template <int XS>
 hipError_t apus_launch_i8_gemv_x(const ApusI8Args &a, hipStream_t st) {
     return a.K > 2048 ? apus_launch_i8_gemv<1, 4, XS>(a, st) : a.K > 1024 ? apus_launch_i8_gemv<2, 2, XS>(a, st)
@@ -555,34 +572,44 @@ hipError_t apus_launch_i8_gemm(const ApusI8Args *a, hipStream_t st) {
     if (a->K % 16 == 0 && (((uintptr_t)a->a | (uintptr_t)a->w) & 15) == 0) {
         if (a->M == 1) return apus_launch_i8_gemv_x<0>(*a, st);
         if (a->M <= 8)
-            return a->O <= 16384 ? apus_launch_i8_narrow<1, 1, 4, 4, true>(*a, st) : apus_launch_i8_narrow<1, 2, 2, 4, true>(*a, st);
-        /* More rows: the schedule whose modelled time is least, R (c steps + e) + t us:
-         * steps of 128 bytes of K, R rounds of the 256 CUs (where two workgroups fit a
-         * CU, the share of a round), c, e and t fitted to 73 measured shapes (rms 8 to 16
-         * % of each; the choice is 2-3 % behind the best of them in the geometric mean). */
+            /* Short rows of many channels: twice the channels a workgroup and half the waves
+             * (16 x 4 / 32 x 2, 8 rows, us: K 1024, 8192 / 16384 / 32768 channels 3.7 / 6.5 / 10.0
+             * against 3.8 / 5.9 / 8.5; K 2048, 12288 channels 6.8 against 7.6; K 4096, 32768 25.8
+             * against 28.6; 4096 x 8192 8.0 against 10.5) */
+            return a->K <= 1024 && a->O > 8192 ? apus_launch_i8_narrow<1, 2, 2, 4, true>(*a, st)
+                                               : apus_launch_i8_narrow<1, 1, 4, 4, true>(*a, st);
+        /* More rows: the schedule whose modelled time is least. n workgroups of `steps`
+         * steps of 128 bytes of K take, in us, rounds of 256 CUs times (c steps + e); where
+         * two workgroups fit a CU, rounds of 512 times (c2 steps + e2), a last one of up to
+         * 256 the former; + t. Fitted to every other of 208 measured shapes (9 to 4096 rows,
+         * 256 to 32768 channels, K 512 to 8192; mean error 4 to 10 % a schedule); on the
+         * rest the choice is 1.9 % behind the fastest of all in the geometric mean, 22 % at
+         * worst. */
         static const struct {
             hipError_t (*launch)(const ApusI8Args &, hipStream_t);
             int bm, bn;
-            bool two;
-            float c, e, t;
+            float c, e, t, c2, e2;
         } sched[] = {
-            {apus_launch_i8_narrow<1, 1, 4, 4, false>, 16, 16, true, 0.059f, 0.59f, 1.86f},
-            {apus_launch_i8_narrow<2, 2, 2, 4, false>, 32, 32, false, 0.140f, 0.72f, 2.13f},
-            {apus_launch_i8_narrow<4, 2, 4, 2, false>, 64, 32, false, 0.170f, 2.37f, 0.62f},
-            {apus_launch_i8_narrow<4, 4, 4, 2, false>, 64, 64, false, 0.243f, 3.99f, 0.63f},
-            {apus_launch_i8_block<ApusI8Blk<64, 64, 4, 2, 4>>, 64, 64, true, 0.306f, 0.58f, 2.95f},
-            {apus_launch_i8_block<ApusI8Blk<64, 128, 2, 4, 4>>, 64, 128, false, 0.439f, 2.72f, 0.95f},
-            {apus_launch_i8_block<ApusI8Blk<128, 128, 2, 4, 4>>, 128, 128, false, 0.574f, 4.38f, 0.53f},
-            {apus_launch_i8_block<ApusI8Blk<128, 128, 2, 4, 2>>, 128, 128, true, 0.697f, 1.84f, 2.53f},
-            {apus_launch_i8_block<ApusI8Blk<256, 256, 2, 4, 2>>, 256, 256, false, 1.391f, 13.74f, -2.19f},
+            {apus_launch_i8_narrow<1, 1, 4, 4, false>, 16, 16, 0.048f, 0.94f, 1.45f, 0.110f, 0.97f},
+            {apus_launch_i8_narrow<2, 2, 2, 4, false>, 32, 32, 0.130f, 0.53f, 2.31f, 0.0f, 0.0f},
+            {apus_launch_i8_narrow<4, 2, 4, 2, false>, 64, 32, 0.158f, 2.27f, 0.79f, 0.0f, 0.0f},
+            {apus_launch_i8_narrow<4, 4, 4, 2, false>, 64, 64, 0.223f, 3.72f, 0.79f, 0.0f, 0.0f},
+            {apus_launch_i8_block<ApusI8Blk<64, 64, 4, 2, 4>>, 64, 64, 0.337f, -0.54f, 3.38f, 0.465f, 1.84f},
+            {apus_launch_i8_block<ApusI8Blk<64, 128, 2, 4, 4>>, 64, 128, 0.426f, 2.71f, 0.82f, 0.0f, 0.0f},
+            {apus_launch_i8_block<ApusI8Blk<128, 128, 2, 4, 4>>, 128, 128, 0.576f, 4.07f, 0.28f, 0.0f, 0.0f},
+            {apus_launch_i8_block<ApusI8Blk<128, 128, 2, 4, 2>>, 128, 128, 0.758f, 1.85f, 1.50f, 1.043f, 4.82f},
+            {apus_launch_i8_block<ApusI8Blk<256, 256, 2, 4, 2>>, 256, 256, 1.406f, 11.76f, -0.52f, 0.0f, 0.0f},
         };
         const float steps = (float)((a->K + 127) / 128);
         int best = 0;
         float least = 0.0f;
         for (int i = 0; i < (int)(sizeof sched / sizeof *sched); ++i) {
-            const size_t wgs = ((size_t)a->M + sched[i].bm - 1) / sched[i].bm * (((size_t)a->O + sched[i].bn - 1) / sched[i].bn);
-            const float r = sched[i].two ? std::max(1.0f, (float)wgs / 256.0f) : (float)((wgs + 255) / 256);
-            const float us = r * (sched[i].c * steps + sched[i].e) + sched[i].t;
+            const auto &c = sched[i];
+            const size_t n = ((size_t)a->M + c.bm - 1) / c.bm * (((size_t)a->O + c.bn - 1) / c.bn);
+            const float one = c.c * steps + c.e, two = c.c2 * steps + c.e2;
+            const size_t left = n % 512;
+            const float us = c.c2 == 0.0f ? (float)((n + 255) / 256) * one + c.t
+                                          : (float)(n / 512) * two + (left == 0 ? 0.0f : left <= 256 ? one : two) + c.t;
             if (i == 0 || us < least) {
                 best = i;
                 least = us;
