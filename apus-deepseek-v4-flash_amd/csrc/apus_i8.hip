@@ -563,13 +563,14 @@ hipError_t apus_launch_i8_gemv_x(const ApusI8Args &a, hipStream_t st) {
 
 /* one row, fp32 or BF16 in: quantised inside the product's launch */
 bool apus_i8_fused_ok(const ApusI8Args *a) {
-    return a->M == 1 && a->K % 16 == 0 && a->K <= 32768 && (((uintptr_t)a->x | (uintptr_t)a->w) & 15) == 0;
+    return a->M == 1 && a->O <= 1 << 26 && a->K % 16 == 0 && a->K <= 32768 && (((uintptr_t)a->x | (uintptr_t)a->w) & 15) == 0;
 }
 
 hipError_t apus_launch_i8_gemm(const ApusI8Args *a, hipStream_t st) {
     if (a->M <= 0) return hipSuccess;
     if (a->x) return a->x_bf16 ? apus_launch_i8_gemv_x<2>(*a, st) : apus_launch_i8_gemv_x<1>(*a, st);
-    if (a->K % 16 == 0 && (((uintptr_t)a->a | (uintptr_t)a->w) & 15) == 0) {
+    /* (more channels than the one-row schedule has workgroups for: the loops of the last kernel) */
+    if (a->K % 16 == 0 && (((uintptr_t)a->a | (uintptr_t)a->w) & 15) == 0 && a->O <= 1 << 26) {
         if (a->M == 1) return apus_launch_i8_gemv_x<0>(*a, st);
         if (a->M <= 8)
             /* Short rows of many channels: twice the channels a workgroup and half the waves

@@ -63,7 +63,9 @@ __device__ __forceinline__ float score32(float z, float zmax) {
         const float d = z - zmax, bb = d - z, r = (z - (d - bb)) + (-zmax - bb);
         return d < -150.0f ? 0.0f : exp32(d, r);
     } else {
-        return sqrtf(fmaxf(z, 0.0f) + log1pf(expf(-fabsf(z))));
+        /* far below zero exp(z) leaves the range before its root does: there the root is
+         * e^(z / 2) within e^z / 4 */
+        return z < -20.0f ? exp32(fmaxf(0.5f * z, -150.0f), 0.0f) : sqrtf(fmaxf(z, 0.0f) + log1pf(expf(-fabsf(z))));
     }
 }
 
@@ -802,7 +804,7 @@ hipError_t apus_launch_route(const ApusRouteArgs *a, hipStream_t st) {
     /* tokens a wave: four waves a SIMD, then more tokens each */
     const int tpw = (int)std::min((size_t)64 / slots, ((size_t)a->s + 4095) / 4096);
     const size_t waves = ((size_t)a->s + tpw - 1) / tpw;
-    const unsigned wgs = (unsigned)std::min((waves + 3) / 4, (size_t)1 << 20);
+    const unsigned wgs = (unsigned)std::min((waves + 3) / 4, (size_t)1024);
     const size_t lds = 4 * (sizeof(WaveLds) + a->E * sizeof(double));
     const bool v = per % (4 * lpg) == 0 && ne <= 16 && al;
     auto go = [&](auto kernel) {

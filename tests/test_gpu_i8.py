@@ -163,3 +163,24 @@ def test_i8_rows_past_32_bits(hip, rng):
         w = dw.to_array(np.int8, (O, K))
         a = np.concatenate([np.ones((1, K), np.int8), tail])
         assert np.array_equal(got, R.bf16_bits(R.product(a, np.ones(4), w, np.ones(O))))
+
+
+def test_i8_more_channels_than_workgroups(hip, rng):
+    """one row and 2^26 + 5 channels: the outputs at both ends"""
+    L = hip.lib()
+    O, K = (1 << 26) + 5, 16
+    dw, da = hip.DevBuf(O * K), hip.DevBuf.from_array(rng.integers(-128, 128, (1, K), dtype=np.int8))
+    hip._check(L.apus_hip_memset(dw.ptr, 3, O * K), "memset")
+    tail = rng.integers(-128, 128, (7, K), dtype=np.int8)
+    hip._check(L.apus_hip_h2d(dw.ptr + (O - 7) * K, tail.ctypes.data, tail.nbytes), "h2d")
+    one = hip.DevBuf.from_array(np.ones(O, np.float32))
+    do = hip.DevBuf(O * 4)
+    hip._check(L.apus_hip_i8_gemm_dev(dw.ptr, one.ptr, da.ptr, one.ptr, do.ptr, 1, O, K, 0), "i8_gemm")
+    hip.synchronize()
+    a = da.to_array(np.int8, (1, K))
+    w = np.concatenate([np.full((5, K), 3, np.int8), tail])
+    want = R.product(a, np.ones(1), w, np.ones(len(w)))[0]
+    head, end = np.empty(5, np.float32), np.empty(7, np.float32)
+    hip._check(L.apus_hip_d2h(head.ctypes.data, do.ptr, head.nbytes), "d2h")
+    hip._check(L.apus_hip_d2h(end.ctypes.data, do.ptr + (O - 7) * 4, end.nbytes), "d2h")
+    assert np.array_equal(head, want[:5]) and np.array_equal(end, want[5:])

@@ -293,3 +293,26 @@ def test_i8_quant_non_finite_row(hip, rng, value, K):
     want, ws = R.quant_i8(R.round_bf16(x[[0, 2]]))
     assert np.array_equal(codes[[0, 2]], want) and np.array_equal(s[[0, 2]], ws)
     assert not codes[1].any() and np.isnan(s[1])
+
+
+def test_rows_in_more_than_one_round(hip, oracle, rng):
+    """more rows than a launch has workgroups for"""
+    M, K = (1 << 20) + 77, 16
+    base = rng.standard_normal((64, K)).astype(np.float32)
+    x = np.tile(base, (M // 64 + 1, 1))[:M]
+    gamma = (1 + 0.3 * rng.standard_normal(K)).astype(np.float32)
+    want = run(hip, oracle, base, None, gamma, "i8", False, False)
+    dx, dg = dev(hip, x), dev(hip, gamma)
+    dc, ds = hip.DevBuf(M * K), hip.DevBuf(M * 4)
+    L = hip.lib()
+    r = np.arange(M) % 64
+    hip._check(L.apus_hip_rmsnorm_dev(dx.ptr, K, None, None, dg.ptr, M, K, EPS, hip.Q_I8, None, dc.ptr, ds.ptr), "norm")
+    assert np.array_equal(dc.to_array(np.int8, (M, K)), want["codes"][r])
+    assert np.array_equal(ds.to_array(np.float32, (M,)), want["scales"][r])
+    for k in (K, 4):                             # 4: the kernel of short rows
+        hip._check(L.apus_hip_i8_quant_dev(dx.ptr, M, k, 0, dc.ptr, ds.ptr), "quant")
+        pieces = base.reshape(-1, k)
+        codes, scales = R.quant_i8(R.round_bf16(pieces))
+        at = np.arange(M) % len(pieces)
+        assert np.array_equal(dc.to_array(np.int8, (M, k)), codes[at])
+        assert np.array_equal(ds.to_array(np.float32, (M,)), scales[at])

@@ -164,3 +164,64 @@ def test_route_many_tokens(hip, rng):
     a, w, _ = call(hip, "sigmoid", z, bias, 6, 8, 4, 2)
     b, v, _ = call(hip, "sigmoid", z[pick], bias, 6, 8, 4, 2)
     assert np.array_equal(b, a[pick]) and np.array_equal(v, w[pick])
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("E,k,groups,keep,top", [(320, 8, 1, 1, 1), (320, 8, 5, 2, 2), (64, 12, 1, 1, 1), (64, 12, 8, 3, 2),
+                                                 (512, 8, 16, 4, 1), (1024, 16, 32, 8, 2), (96, 6, 3, 2, 1)])
+def test_route_ties_and_masks_other_shapes(hip, rng, kind, E, k, groups, keep, top):
+    """many experts, many of them chosen, group counts that do not divide a row of 16 lanes"""
+    z = logits(rng, 40, E)
+    z[:12] = np.round(2 * z[:12]) / 2
+    z[3] = 0.25
+    z[4, ::2] = 1.0
+    z[4, 1::2] = 1.0 + 2.0 ** -23
+    z[12] = -np.inf
+    z[13] = np.nan
+    z[14, 5:] = -np.inf
+    z[15, ::2] = np.nan
+    z[16, E // 8:] = -np.inf
+    z[17] = -3.4028235e38
+    z[18, 1::2] = -3.4028235e38
+    z[19, [2, 9, E - 1]] = np.inf
+    z[20] = -800.0
+    z[21, :E - 1] = -np.inf
+    check(hip, kind, z, None, k, groups, keep, top)
+    bias = (np.round(4 * rng.standard_normal(E)) / 64).astype(np.float32)
+    check(hip, kind, z, bias, k, groups, keep, top)
+    bias[[1, 17, 40]] = -np.inf
+    bias[50] = np.nan
+    bias[33] = np.inf
+    idx, wgt = check(hip, kind, z, bias, k, groups, keep, top, renorm=0, scale=1.0)
+    assert np.isfinite(wgt).all()
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("groups,keep,top", [(1, 1, 1), (8, 3, 2), (16, 5, 1)])
+@pytest.mark.parametrize("shift,spread", [(-60.0, 3.0), (-20.0, 1.0), (-6.0, 0.01), (0.0, 1e-4), (0.0, 1e-6), (12.0, 0.5),
+                                          (60.0, 5.0), (0.0, 40.0), (1e4, 1e3), (-3.0, 1e-3)])
+def test_route_where_fp32_tells_little(hip, rng, kind, groups, keep, top, shift, spread):
+    """scores that are tiny, saturated or closer than their rounding, with and without a
+    bias that swamps or cancels them: the choice stays that of the 64-bit values"""
+    E = 256
+    z = (shift + spread * rng.standard_normal((24, E))).astype(np.float32)
+    check(hip, kind, z, None, 8, groups, keep, top, least=0.0)
+    for scale in (1e-6, 1.0, 300.0):
+        check(hip, kind, z, (scale * rng.standard_normal(E)).astype(np.float32), 8, groups, keep, top, least=0.0)
+    p, _ = R.scores(kind, z[:1])
+    check(hip, kind, z, -p[0].astype(np.float32), 8, groups, keep, top, least=0.0)
+
+
+def test_route_many_tokens_many_experts(hip, rng):
+    E, s = 320, 40000
+    z = logits(rng, 400, E)
+    pick = rng.integers(0, 400, s)
+    a, w, _ = call(hip, "softmax", z, None, 8, want_scores=False)
+    b, v, _ = call(hip, "softmax", z[pick], None, 8, want_scores=False)
+    assert np.array_equal(b, a[pick]) and np.array_equal(v, w[pick])
+
+
+def test_route_no_tokens(hip):
+    cfg = hip.ApusHipRoute(1, 2, 1, 1, 1, 1, 1.0)
+    b = hip.DevBuf(64)
+    assert hip.lib().apus_hip_route_dev(C.byref(cfg), b.ptr, None, 0, 4, b.ptr + 16, b.ptr + 32, None) == 0
