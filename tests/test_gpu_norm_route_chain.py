@@ -106,10 +106,10 @@ def test_chain_against_the_formulas(layer, hip, oracle):
     # the FP8 product and the experts on codes, ids and weights computed apart
     up = hip.DevBuf.from_array
     L, s = layer.L, layer.s
-    kc, ks, ki, kw = up(c8), up(s8), up(idx), up(o["wgt"])
+    kc, ks, ki, kw, ky = up(c8), up(s8), up(idx), up(o["wgt"]), up(o["y"])
     o8, ym = hip.DevBuf(s * 512 * 4), hip.DevBuf(s * DIM * 4)
     hip._check(L.apus_hip_fp8_gemm_dev(layer.w8.ptr, layer.w8s.ptr, kc.ptr, ks.ptr, o8.ptr, s, 512, DIM, 0), "fp8")
-    hip._check(L.apus_hip_moe_routed_dev(layer.store, 0, up(o["y"]).ptr, ki.ptr, kw.ptr, s, TOPK, 10.0, ym.ptr,
+    hip._check(L.apus_hip_moe_routed_dev(layer.store, 0, ky.ptr, ki.ptr, kw.ptr, s, TOPK, 10.0, ym.ptr,
                                          layer.ws.ptr), "experts")
     hip.synchronize()
     assert np.array_equal(o8.to_array(np.float32, (s, 512)), o["o8"])
