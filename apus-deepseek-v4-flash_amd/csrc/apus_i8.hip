@@ -119,13 +119,15 @@ __global__ __launch_bounds__(256) void apus_i8_any_kernel(ApusI8Args a) {
  * outputs of one row. Rows past M or O repeat the last one; past K the activations are
  * zeroed in LDS (0 times whatever the clamped weight bytes are).
  * 4096 x 8192 x 4096, 256 x 256 tiles: 122-127 us, 2.2 POP/s (a large library product of
- * these sizes 130); the matrix cores are busy 49 % of its cycles at 2.1 GHz (the rest
- * follows the barrier: the stage's wait, the skew of 8 waves), the 64 MB of outputs go out
- * in two bursts. 1000 x 4096 x 8192, 128 x 128 tiles four stages deep: 46 us, one wave of
- * tiles whose operand stream L2 -> LDS runs at 14 TB/s, about what all tiles reach.
- * Outputs straight from registers 191 us instead of 129 (stores of 8 bytes to 16 rows);
- * 32x32x32 instructions 139 (fragments of half the depth); the wave's priority raised around
- * the instructions 130, and 45.7 for 46.8 with 128 x 128 tiles: not kept.
+ * these sizes 130); the matrix cores are busy 49 % of its cycles at 2.1 GHz, without loads it
+ * takes 15 % less, with the matrix instructions and barriers alone 30 %; the 64 MB of outputs
+ * go out in two bursts. 1000 x 4096 x 8192, 128 x 128 tiles four stages deep, one round: 42 us
+ * (46 with a step's loads in a burst behind its barrier); without loads 35, the matrix
+ * instructions and barriers alone 29, the loads alone 26 (22 TB/s out of L2). Tried there: 4
+ * waves of 64 x 64 56, 16 waves 46; two waves on the halves of each step's K, for two thirds of
+ * the fragment reads, 42; one barrier for two steps 51. Outputs straight from registers
+ * (4096 x 8192 x 4096) 191 instead of 129 (stores of 8 bytes to 16 rows); 32x32x32 instructions
+ * 139 (fragments of half the depth); the wave's priority raised around the instructions 130.
  */
 template <int BM_, int BN_, int WM_, int WN_, int NST_>
 struct ApusI8Blk {
@@ -152,63 +154,71 @@ __global__ __launch_bounds__(64 * B::NW) void apus_i8_block_kernel(ApusI8Args a)
      * row's last chunk */
     const uint8_t *xb = (const uint8_t *)a.a + (size_t)m0 * K, *wb = (const uint8_t *)a.w + (size_t)n0 * K;
     unsigned off[B::LPW];
-    int chunk[B::LPW];
     auto load_of = [&](int u) { return min(wave * B::LPW + u, B::LT - 1); };
+    /* the lane's chunk of row 8 j + lane / 8, j = load_of(u) or, of a weight, an even LX less */
+    auto chunk_in = [&](int u) { return (lane & 7) ^ ((4 * load_of(u) + (lane >> 4)) & 7); };
 #pragma unroll
     for (int u = 0; u < B::LPW; ++u) {
         const int ii = load_of(u), i = 8 * (ii < B::LX ? ii : ii - B::LX) + (lane >> 3);
-        chunk[u] = (lane & 7) ^ ((i >> 1) & 7);
-        off[u] = (unsigned)min(i, (ii < B::LX ? a.M - m0 : a.O - n0) - 1) * (unsigned)K + chunk[u] * 16;
+        off[u] = (unsigned)min(i, (ii < B::LX ? a.M - m0 : a.O - n0) - 1) * (unsigned)K + chunk_in(u) * 16;
     }
+    auto issue1 = [&](int u, int q, int slot, bool last) {
+        const int ii = load_of(u);
+        unsigned o = off[u];
+        if (last) o -= max(0, chunk_in(u) * 16 - (tail - 16));
+        asm("" : "+v"(o));                                   /* 32 bits beside the uniform base */
+        apus_g2lds16((ii < B::LX ? xb : wb) + (size_t)q * 128 + o, lbase + slot * B::STB + ii * 1024);
+    };
     auto issue = [&](int q, int slot) {
         const bool last = tail && q == nq - 1;
 #pragma unroll
-        for (int u = 0; u < B::LPW; ++u) {
-            const int ii = load_of(u);
-            unsigned o = off[u];
-            if (last) o -= max(0, chunk[u] * 16 - (tail - 16));
-            asm("" : "+v"(o));                                   /* 32 bits beside the uniform base */
-            apus_g2lds16((ii < B::LX ? xb : wb) + (size_t)q * 128 + o, lbase + slot * B::STB + ii * 1024);
-        }
+        for (int u = 0; u < B::LPW; ++u) issue1(u, q, slot, last);
     };
     /* the activation chunks past K that this wave loaded, once they are in LDS */
     auto zero_tail = [&](int slot) {
 #pragma unroll
         for (int u = 0; u < B::LPW; ++u)
-            if (load_of(u) < B::LX && chunk[u] * 16 >= tail)
+            if (load_of(u) < B::LX && chunk_in(u) * 16 >= tail)
                 *reinterpret_cast<apus_v4i *>(lds + slot * B::STB + load_of(u) * 1024 + lane * 16) = apus_v4i{0, 0, 0, 0};
     };
     struct Frag { apus_v4i w[TN], x[TM]; };
     const int sw = (r >> 1) & 7;
-    auto read = [&](Frag &f, int slot, int s) {
-        const uint8_t *stg = lds + slot * B::STB;
-        const int c = ((4 * s + g) ^ sw) << 4;
-#pragma unroll
-        for (int i = 0; i < TN; ++i)
-            f.w[i] = *reinterpret_cast<const apus_v4i *>(stg + (B::BM + (wn * TN + i) * 16 + r) * 128 + c);
-#pragma unroll
-        for (int t = 0; t < TM; ++t)
-            f.x[t] = *reinterpret_cast<const apus_v4i *>(stg + ((wm * TM + t) * 16 + r) * 128 + c);
+    /* fragment j of half s of a stage: the weights', then the activations' */
+    auto read1 = [&](Frag &f, int j, const uint8_t *stg, int c) {
+        if (j < TN) f.w[j] = *reinterpret_cast<const apus_v4i *>(stg + (B::BM + (wn * TN + j) * 16 + r) * 128 + c);
+        else        f.x[j - TN] = *reinterpret_cast<const apus_v4i *>(stg + ((wm * TM + j - TN) * 16 + r) * 128 + c);
     };
+    auto chunk_of = [&](int s) { return ((4 * s + g) ^ sw) << 4; };
     apus_v4i acc[TN][TM];
 #pragma unroll
     for (int i = 0; i < TN; ++i)
 #pragma unroll
         for (int t = 0; t < TM; ++t) acc[i][t] = apus_v4i{0, 0, 0, 0};
-    auto mul = [&](const Frag &f) {
+    /* Products of half a stage, and among them the reads of the next half's fragments and
+     * (load) the wave's loads of stage q: a wave issues in order, and in a burst behind the
+     * barrier its loads wait for the address unit while no matrix instruction goes out */
+    auto half = [&](const Frag &now, Frag &next, int from, int s, bool more, bool load, int q, int to, bool last) {
+        constexpr int NM = TN * TM, NR = TN + TM, P = NM < B::LPW ? NM : B::LPW;
+        const uint8_t *stg = lds + from * B::STB;
+        const int c = chunk_of(s);
+        auto one = [&](int j) {
+            acc[j / TM][j % TM] = __builtin_amdgcn_mfma_i32_16x16x64_i8(now.w[j / TM], now.x[j % TM], acc[j / TM][j % TM], 0, 0, 0);
+        };
 #pragma unroll
-        for (int i = 0; i < TN; ++i)
+        for (int p = 0; p < P; ++p) {
+            one(p * NM / P);
+            __builtin_amdgcn_sched_barrier(0);
+            if (load) {
 #pragma unroll
-            for (int t = 0; t < TM; ++t)
-                acc[i][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f.w[i], f.x[t], acc[i][t], 0, 0, 0);
-    };
-    /* the fragment reads spread among the matrix instructions */
-    auto weave = [&]() {
-        constexpr int NR = TM + TN, NM = TM * TN, PER = (NR + NM - 1) / NM;
+                for (int u = p * B::LPW / P; u < (p + 1) * B::LPW / P; ++u) issue1(u, q, to, last);
+            }
+            if (more) {
 #pragma unroll
-        for (int i = 0; i < NM; ++i) {
-            __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                for (int j = p * NR / P; j < (p + 1) * NR / P; ++j) read1(next, j, stg, c);
+            }
+#pragma unroll
+            for (int j = p * NM / P + 1; j < (p + 1) * NM / P; ++j) one(j);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
     /* scales of the block's rows, then of its columns, to LDS */
@@ -231,25 +241,21 @@ __global__ __launch_bounds__(64 * B::NW) void apus_i8_block_kernel(ApusI8Args a)
     };
     arrive(0, 0, pre);
     Frag fr[2];
-    read(fr[0], 0, 0);
+#pragma unroll
+    for (int j = 0; j < TN + TM; ++j) read1(fr[0], j, lds, chunk_of(0));
     int slot = 0;
-    for (int q = 0; q < nq; ++q) {
+    /* stage q, whose first half is in fr[0] */
+    auto step = [&](int q, bool more, bool load, bool last) {
         const int nxt = slot + 1 == NST ? 0 : slot + 1;
-        read(fr[1], slot, 1);
-        mul(fr[0]);
-        weave();
+        half(fr[0], fr[1], slot, 1, true, false, 0, 0, false);
+        if (more) arrive(q + 1, nxt, min(nq, q + NST));
         __builtin_amdgcn_sched_barrier(0);
-        if (q + 1 < nq) {
-            arrive(q + 1, nxt, min(nq, q + NST));
-            if (q + NST < nq) issue(q + NST, slot);
-            __builtin_amdgcn_sched_barrier(0);
-            read(fr[0], nxt, 0);
-        }
-        mul(fr[1]);
-        weave();
-        __builtin_amdgcn_sched_barrier(0);
+        half(fr[1], fr[0], nxt, 0, more, load, q + NST, slot, last);
         slot = nxt;
-    }
+    };
+    int q = 0;
+    for (; q + 1 + NST < nq; ++q) step(q, true, true, false);
+    for (; q < nq; ++q) step(q, q + 1 < nq, q + NST < nq, tail && q + NST == nq - 1);
     /* Outputs: 16 rows at a time through a wave's own LDS, so that a store writes whole
      * lines. A lane holds row r, columns 4 g .. 4 g + 3 of each tile. */
     constexpr int E = YB ? 2 : 4, CW = TN * 16, PITCH = CW * E + 16;
@@ -582,24 +588,24 @@ hipError_t apus_launch_i8_gemm(const ApusI8Args *a, hipStream_t st) {
         /* More rows: the schedule whose modelled time is least. n workgroups of `steps`
          * steps of 128 bytes of K take, in us, rounds of 256 CUs times (c steps + e); where
          * two workgroups fit a CU, rounds of 512 times (c2 steps + e2), a last one of up to
-         * 256 the former; + t. Fitted to every other of 208 measured shapes (9 to 4096 rows,
-         * 256 to 32768 channels, K 512 to 8192; mean error 4 to 10 % a schedule); on the
-         * rest the choice is 1.9 % behind the fastest of all in the geometric mean, 22 % at
-         * worst. */
+         * 256 the former; + t. Fitted to every other of 228 measured shapes (9 to 4096 rows,
+         * 256 to 32768 channels, K 512 to 8192; mean error 6 to 11 % a schedule); on the
+         * rest the choice is 0.7 % behind the fastest of all in the geometric mean, 12 % at
+         * worst. Without 256 x 128 it is 0.8 %, 23 % at worst; without any other, 1.0 to 8.2 %. */
         static const struct {
             hipError_t (*launch)(const ApusI8Args &, hipStream_t);
             int bm, bn;
             float c, e, t, c2, e2;
         } sched[] = {
-            {apus_launch_i8_narrow<1, 1, 4, 4, false>, 16, 16, 0.048f, 0.94f, 1.45f, 0.110f, 0.97f},
-            {apus_launch_i8_narrow<2, 2, 2, 4, false>, 32, 32, 0.130f, 0.53f, 2.31f, 0.0f, 0.0f},
-            {apus_launch_i8_narrow<4, 2, 4, 2, false>, 64, 32, 0.158f, 2.27f, 0.79f, 0.0f, 0.0f},
-            {apus_launch_i8_narrow<4, 4, 4, 2, false>, 64, 64, 0.223f, 3.72f, 0.79f, 0.0f, 0.0f},
-            {apus_launch_i8_block<ApusI8Blk<64, 64, 4, 2, 4>>, 64, 64, 0.337f, -0.54f, 3.38f, 0.465f, 1.84f},
-            {apus_launch_i8_block<ApusI8Blk<64, 128, 2, 4, 4>>, 64, 128, 0.426f, 2.71f, 0.82f, 0.0f, 0.0f},
-            {apus_launch_i8_block<ApusI8Blk<128, 128, 2, 4, 4>>, 128, 128, 0.576f, 4.07f, 0.28f, 0.0f, 0.0f},
-            {apus_launch_i8_block<ApusI8Blk<128, 128, 2, 4, 2>>, 128, 128, 0.758f, 1.85f, 1.50f, 1.043f, 4.82f},
-            {apus_launch_i8_block<ApusI8Blk<256, 256, 2, 4, 2>>, 256, 256, 1.406f, 11.76f, -0.52f, 0.0f, 0.0f},
+            {apus_launch_i8_narrow<1, 1, 4, 4, false>, 16, 16, 0.046f, 1.04f, 1.46f, 0.105f, 0.99f},
+            {apus_launch_i8_narrow<2, 2, 2, 4, false>, 32, 32, 0.129f, 0.54f, 2.31f, 0.0f, 0.0f},
+            {apus_launch_i8_narrow<4, 2, 4, 2, false>, 64, 32, 0.159f, 2.23f, 0.81f, 0.0f, 0.0f},
+            {apus_launch_i8_block<ApusI8Blk<64, 64, 4, 2, 4>>, 64, 64, 0.216f, 1.00f, 2.48f, 0.419f, 2.42f},
+            {apus_launch_i8_block<ApusI8Blk<64, 128, 2, 4, 4>>, 64, 128, 0.352f, 3.24f, 0.55f, 0.0f, 0.0f},
+            {apus_launch_i8_block<ApusI8Blk<128, 128, 2, 4, 4>>, 128, 128, 0.481f, 5.69f, -1.01f, 0.0f, 0.0f},
+            {apus_launch_i8_block<ApusI8Blk<128, 128, 2, 4, 2>>, 128, 128, 0.779f, 0.12f, 3.03f, 1.020f, 4.95f},
+            {apus_launch_i8_block<ApusI8Blk<256, 128, 4, 2, 3>>, 256, 128, 0.797f, 7.71f, -0.71f, 0.0f, 0.0f},
+            {apus_launch_i8_block<ApusI8Blk<256, 256, 2, 4, 2>>, 256, 256, 1.403f, 13.47f, -3.17f, 0.0f, 0.0f},
         };
         const float steps = (float)((a->K + 127) / 128);
         int best = 0;
