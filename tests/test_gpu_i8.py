@@ -73,6 +73,19 @@ def test_i8_many_rows(hip, rng, M, O, K, bf):
     check(hip, rng, M, O, K, hip.Y_BF16 if bf else 0)
 
 
+@pytest.mark.parametrize("M,O", [(777, 4225), (8205, 131), (1671, 1414), (8445, 401), (8300, 70)])
+@pytest.mark.parametrize("K", [16, 112, 128, 144, 256, 272, 400, 512, 560, 656, 1152])
+def test_i8_ragged_tiles(hip, rng, M, O, K):
+    """more and fewer steps of K than a tile's loads under way, whole and ragged last steps,
+    rows and channels that end inside a tile, of each tile size"""
+    check(hip, rng, M, O, K, hip.Y_BF16 if K % 3 else 0)
+
+
+@pytest.mark.parametrize("M,O,K", [(2690, 4369, 112), (1420, 8231, 496), (775, 9381, 1072), (1675, 6933, 640)])
+def test_i8_ragged_largest_tiles(hip, rng, M, O, K):
+    check(hip, rng, M, O, K, 0 if K % 128 else hip.Y_BF16)
+
+
 @pytest.mark.parametrize("offs", [(4, 0, 0), (0, 4, 0), (0, 0, 4), (8, 8, 8), (12, 4, 12)])
 @pytest.mark.parametrize("M", [1, 5, 20, 200])
 def test_i8_alignment(hip, rng, offs, M):
