@@ -71,8 +71,9 @@ __device__ __forceinline__ void apus_i8_tile(unsigned b, int mt, int nt, int &mb
 
 }  // namespace
 
-/* Any shape with K % 4 == 0, 4-byte alignment: 64 x 64 outputs a workgroup,
- * 4 x 4 a thread, steps of 64 bytes of K through LDS. */
+/* K % 16 != 0 or codes not 16-byte aligned (K % 4 == 0, 4-byte alignment): 64 x 64 outputs a
+ * workgroup, 4 x 4 a thread, steps of 64 bytes of K through LDS, dot products on the vector
+ * units. 4096 x 8192 x 4096 1546 us (121-127 with 16-byte pieces), 40 x 32768 x 1024 47 (8.5). */
 template <bool YB>
 __global__ __launch_bounds__(256) void apus_i8_any_kernel(ApusI8Args a) {
     __shared__ int la[64][17], lw[64][17];
@@ -119,7 +120,7 @@ __global__ __launch_bounds__(256) void apus_i8_any_kernel(ApusI8Args a) {
  * outputs of one row. Rows past M or O repeat the last one; past K the activations are
  * zeroed in LDS (0 times whatever the clamped weight bytes are).
  * 4096 x 8192 x 4096, 256 x 256 tiles: 122-127 us, 2.2 POP/s (a large library product of
- * these sizes 130); the matrix cores are busy 49 % of its cycles at 2.1 GHz, without loads it
+ * these sizes 130); the matrix cores are busy 49-51 % of its cycles at 2.1 GHz, without loads it
  * takes 15 % less, with the matrix instructions and barriers alone 30 %; the 64 MB of outputs
  * go out in two bursts. 1000 x 4096 x 8192, 128 x 128 tiles four stages deep, one round: 42 us
  * (46 with a step's loads in a burst behind its barrier); without loads 35, the matrix

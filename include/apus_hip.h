@@ -395,7 +395,7 @@ int apus_hip_rmsnorm_dev(const void *x, int ldx, const void *res, void *res_out,
  *     p with renorm) * route_scale
  * The choice and the weights are those of 64-bit p and sel, so they do not depend on
  * how an exponential was rounded; ties (experts or groups) go to the lowest index.
- * scores [s, E], if given, receives p of every expert in fp32, within 2^-21. Experts whose logit
+ * scores [s, E], if given, receives p of every expert in fp32, within 2^-21 p + 2^-125. Experts whose logit
  * or bias is -inf or NaN are masked: chosen last, lowest index first, with weight
  * 0 (and left out of a group's sum); their p is 0 where the logit masks them. A
  * weight sum of 0 gives zeros. +inf is read as the largest fp32.
