@@ -10,6 +10,11 @@
 #include <algorithm>
 
 typedef int apus_v4i __attribute__((ext_vector_type(4)));
+/* the vector unit takes 8- and 16-byte accesses at any address (2997 x 18270 x 112, BF16 rows of
+ * outputs of no whole 16 bytes: 42 us, element by element 124) */
+typedef unsigned apus_v4u_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned apus_v2u_any __attribute__((ext_vector_type(2), aligned(2)));
+typedef float apus_v4f_any __attribute__((ext_vector_type(4), aligned(4)));
 
 namespace {
 
@@ -29,14 +34,13 @@ __device__ __forceinline__ uint64_t bf16x4(const float (&v)[4]) {
            (uint64_t)apus_bf16_bits(v[3]) << 48;
 }
 
-/* outputs (m, o .. o + 3): one store where the row's pieces are aligned for it */
+/* outputs (m, o .. o + 3) */
 template <bool YB>
 __device__ __forceinline__ void i8_store4(const ApusI8Args &a, int m, int o, apus_v4i acc) {
-    constexpr int E = YB ? 2 : 4;
     const float sa = a.as[m];
     const size_t i = (size_t)m * a.O + o;
-    if (((a.O * (size_t)E | (uintptr_t)a.out) & (4 * E - 1)) == 0 && ((uintptr_t)a.ws & 15) == 0 && o < a.O) {
-        const apus_v4f sw = *reinterpret_cast<const apus_v4f *>(a.ws + o);
+    if (o + 4 <= a.O) {
+        const apus_v4f_any sw = *(const APUS_GLOBAL apus_v4f_any *)(a.ws + o);
         float v[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -44,9 +48,9 @@ __device__ __forceinline__ void i8_store4(const ApusI8Args &a, int m, int o, apu
             if (YB || a.round_out) v[k] = apus_bf16_rne(v[k]);
         }
         if constexpr (YB)
-            apus_gst<uint64_t>((uint16_t *)a.out + i, bf16x4(v));
+            *(APUS_GLOBAL apus_v2u_any *)((uint16_t *)a.out + i) = __builtin_bit_cast(apus_v2u_any, bf16x4(v));
         else
-            apus_gst<apus_v4f>((float *)a.out + i, apus_v4f{v[0], v[1], v[2], v[3]});
+            *(APUS_GLOBAL apus_v4f_any *)((float *)a.out + i) = apus_v4f_any{v[0], v[1], v[2], v[3]};
         return;
     }
 #pragma unroll
@@ -270,7 +274,7 @@ __global__ __launch_bounds__(64 * B::NW) void apus_i8_block_kernel(ApusI8Args a)
 #pragma unroll
     for (int i = 0; i < TN; ++i) sw4[i] = *reinterpret_cast<const apus_v4f *>(lws + i * 16 + 4 * g);
     const int col = n0 + wn * CW + lane % LR * (16 / E);
-    const bool whole = ((a.O * (size_t)E | (uintptr_t)a.out) & 15) == 0 && col + 16 / E <= a.O;
+    const bool whole = col + 16 / E <= a.O;
 #pragma unroll
     for (int t = 0; t < TM; ++t) {
         const float sa = las[t * 16 + r];
@@ -294,7 +298,7 @@ __global__ __launch_bounds__(64 * B::NW) void apus_i8_block_kernel(ApusI8Args a)
             const apus_v4u v = *reinterpret_cast<const apus_v4u *>(ob + row * PITCH + lane % LR * 16);
             uint8_t *d = (uint8_t *)a.out + ((size_t)m * a.O + col) * E;
             if (m < a.M && whole) {
-                apus_gst<apus_v4u>(d, v);
+                *(APUS_GLOBAL apus_v4u_any *)d = v;
             } else if (m < a.M) {
 #pragma unroll
                 for (int k = 0; k < 16 / E; ++k)
