@@ -165,8 +165,8 @@ __device__ __forceinline__ unsigned pk_i8(float a, float b, float c, float d, fl
 }
 
 /*
- * Rows of 8 to 8 C TPR elements: TPR threads a row, 8 neighbouring elements a thread
- * and chunk, the row and the thread's part of gamma in registers, rows in a stride.
+ * Rows of 8 to 8 C TPR elements: TPR threads a row (16 or 32: several rows a wave), 8
+ * neighbouring elements a thread and chunk, the row and the thread's part of gamma in registers, rows in a stride.
  * A chunk past the row's end, or over it where K is no multiple of 8, is the row's
  * last 8 elements again: they are left out of the sum, and what is stored twice is
  * the same. Every store comes after the barrier behind all loads of the row, so
@@ -174,7 +174,7 @@ __device__ __forceinline__ unsigned pk_i8(float a, float b, float c, float d, fl
  */
 template <int TPR, int C, bool XB, bool YB>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void apus_rmsnorm_kernel(ApusNormArgs a) {
-    constexpr int NT = TPR < 256 ? 256 : TPR, RPB = NT / TPR, NWR = TPR / 64;
+    constexpr int NT = TPR < 256 ? 256 : TPR, RPB = NT / TPR, NWR = (TPR + 63) / 64, HALF = TPR < 64 ? TPR / 2 : 32;
     const int tid = threadIdx.x % TPR, lane = threadIdx.x & 63, wr = tid >> 6;
     const int K = a.K;
     __shared__ double lss[2][NWR];
@@ -254,7 +254,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void apus_rmsnorm_kernel(Apu
             ss += s;
         }
 #pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) ss += __shfl_xor(ss, o, 64);
+        for (int o = HALF; o >= 1; o >>= 1) ss += __shfl_xor(ss, o, 64);
         if constexpr (NWR > 1) {
             if (lane == 0) lss[flip][wr] = ss;
             __syncthreads();
@@ -298,7 +298,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void apus_rmsnorm_kernel(Apu
 #pragma unroll
                 for (int j = 0; j < 4; ++j) mx = max(mx, max(b[c][j] & 0x7fffu, (b[c][j] >> 16) & 0x7fffu));
 #pragma unroll
-            for (int o = 32; o >= 1; o >>= 1) mx = max(mx, (unsigned)__shfl_xor((int)mx, o, 64));
+            for (int o = HALF; o >= 1; o >>= 1) mx = max(mx, (unsigned)__shfl_xor((int)mx, o, 64));
             if constexpr (NWR > 1) {
                 if (lane == 0) lmx[flip][wr] = mx;
                 __syncthreads();
@@ -345,6 +345,9 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void apus_rmsnorm_kernel(Apu
 
 /* Threads a row and chunks a thread (us, BF16 in and out, residual, y and codes, one row /
  * 512 / 8192 rows unless said):
+ *   K = 44     (25011 rows, fp32, codes alone) 16 x 1 5.6   32 x 1 8.8   64 x 1 14.8
+ *   K = 128    16 x 1  2.4 / -   / 4.3     32 x 1   2.4 / -   / 5.0     64 x 1   2.5 / -   / 7.4
+ *   K = 256    32 x 1  2.4 / -   / 6.8     64 x 1   2.4 / -   / 8.8     16 x 2   2.8 / -   / 6.6
  *   K = 512    64 x 1  2.4 / 3.1 / 11.7    64 x 2   2.9 / 3.5 / 12.9    256 x 1  2.7 / 3.7 / 22.9
  *   K = 1024   64 x 2  2.9 / 3.9 / 18.4    64 x 4   4.1 / 5.1 / 24.8    256 x 1  2.8 / 4.0 / 25.1
  *   K = 2048   256 x 1 2.8 / 4.7 / 31.3    64 x 4   4.1 / 5.7 / 32.5    256 x 2  3.2 / 5.3 / 38.9
@@ -362,6 +365,8 @@ hipError_t apus_launch_rmsnorm_t(const ApusNormArgs &a, hipStream_t st) {
         return hipGetLastError();
     };
     if (a.K < 8 || a.K > 16384) return go(apus_rmsnorm_any_kernel<XB, YB>, 256, 1);
+    if (a.K <= 128)  return go(apus_rmsnorm_kernel<16, 1, XB, YB>, 256, 16);
+    if (a.K <= 256)  return go(apus_rmsnorm_kernel<32, 1, XB, YB>, 256, 8);
     if (a.K <= 512)  return go(apus_rmsnorm_kernel<64, 1, XB, YB>, 256, 4);
     if (a.K <= 1024) return go(apus_rmsnorm_kernel<64, 2, XB, YB>, 256, 4);
     if (a.K <= 2048) return go(apus_rmsnorm_kernel<256, 1, XB, YB>, 256, 1);
@@ -407,7 +412,7 @@ template <int TPR, int C, bool XB>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void apus_i8_quant_kernel(const void *__restrict__ x, int M, int K,
                                                                               int8_t *__restrict__ codes,
                                                                               float *__restrict__ scales) {
-    constexpr int NT = TPR < 256 ? 256 : TPR, RPB = NT / TPR, NWR = TPR / 64;
+    constexpr int NT = TPR < 256 ? 256 : TPR, RPB = NT / TPR, NWR = (TPR + 63) / 64, HALF = TPR < 64 ? TPR / 2 : 32;
     const int tid = threadIdx.x % TPR, lane = threadIdx.x & 63, wr = tid >> 6;
     __shared__ unsigned lmx[2][NWR];
     int flip = 0;
@@ -428,7 +433,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void apus_i8_quant_kernel(co
             }
         }
 #pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) mx = max(mx, (unsigned)__shfl_xor((int)mx, o, 64));
+        for (int o = HALF; o >= 1; o >>= 1) mx = max(mx, (unsigned)__shfl_xor((int)mx, o, 64));
         if constexpr (NWR > 1) {
             if (lane == 0) lmx[flip][wr] = mx;
             __syncthreads();
@@ -460,6 +465,8 @@ hipError_t apus_launch_i8_quant_t(const void *x, int M, int K, int8_t *codes, fl
         return hipGetLastError();
     };
     if (K < 8 || K > 16384) return go(apus_i8_quant_any_kernel<XB>, 256, 1);
+    if (K <= 128)  return go(apus_i8_quant_kernel<16, 1, XB>, 256, 16);
+    if (K <= 256)  return go(apus_i8_quant_kernel<32, 1, XB>, 256, 8);
     if (K <= 512)  return go(apus_i8_quant_kernel<64, 1, XB>, 256, 4);
     if (K <= 1024) return go(apus_i8_quant_kernel<64, 2, XB>, 256, 4);
     if (K <= 2048) return go(apus_i8_quant_kernel<256, 1, XB>, 256, 1);

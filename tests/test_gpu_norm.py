@@ -316,3 +316,27 @@ def test_rows_in_more_than_one_round(hip, oracle, rng):
         at = np.arange(M) % len(pieces)
         assert np.array_equal(dc.to_array(np.int8, (M, k)), codes[at])
         assert np.array_equal(ds.to_array(np.float32, (M,)), scales[at])
+
+
+@pytest.mark.parametrize("K", [8, 9, 15, 44, 120, 127, 128, 129, 136, 200, 255, 256, 257])
+@pytest.mark.parametrize("M", [1, 7, 16, 33, 700])
+@pytest.mark.parametrize("bf", [False, True])
+def test_several_short_rows_a_wave(hip, oracle, rng, K, M, bf):
+    """rows that share a wave, the last wave not full; a non-finite row beside the others"""
+    for quant in (["e4m3", "i8"] if K % 128 == 0 else ["i8", None]):
+        run(hip, oracle, *inputs(rng, M, K, True), quant, bf, bf)
+    x = rng.standard_normal((M, K)).astype(np.float32)
+    x[M // 2, K // 3] = np.nan
+    dx, dg = hip.DevBuf.from_array(x), hip.DevBuf.from_array(np.ones(K, np.float32))
+    dc, ds = hip.DevBuf(M * K), hip.DevBuf(M * 4)
+    L = hip.lib()
+    for norm in (True, False):
+        if norm:
+            hip._check(L.apus_hip_rmsnorm_dev(dx.ptr, K, None, None, dg.ptr, M, K, EPS, hip.Q_I8, None, dc.ptr, ds.ptr), "norm")
+        else:
+            hip._check(L.apus_hip_i8_quant_dev(dx.ptr, M, K, 0, dc.ptr, ds.ptr), "quant")
+        hip.synchronize()
+        c, s = dc.to_array(np.int8, (M, K)), ds.to_array(np.float32, (M,))
+        bad = np.arange(M) == M // 2
+        assert np.isnan(s[bad]).all() and not c[bad].any() and (s[~bad] > 0).all()
+        assert (np.abs(c[~bad]).max(1, initial=0) == 127).all()
