@@ -476,8 +476,8 @@ namespace {
 /* p in fp32 from the bare instructions (softmax: without the sum): where no scores are
  * asked for, only its order counts. Absolute error, with x = |z| or zmax - z, exponents
  * within (x + 2) 2^-24 relative: sigmoid p (1 - p) (x + 2) 2^-24 + 2^-23 p < 2^-22;
- * softmax e^-x (2 x + 3) 2^-24 < 2^-22; sqrt-softplus 2^-22 / (2 p) + 2^-23 p, below 2^-20
- * from p = 0.25 on, and 2^-12 at most. */
+ * softmax e^-x (2 x + 3) 2^-24 < 2^-22; sqrt-softplus 2^-22 / (2 p) + 1.25 * 2^-23 p, of
+ * which the first is 2^-21 at most from p = 0.25 on, and 2^-12 at most below. */
 template <int KIND>
 __device__ __forceinline__ float quick32(float z, float zmax) {
     const float L = 1.44269504f;
@@ -681,10 +681,14 @@ __global__ __launch_bounds__(256) void apus_route_row_kernel(ApusRouteArgs a, in
             r2 += x2 > m2 ? 1 : 0;
         });
         float thr = -row_max(fmaxf(r1 < k ? -m1 : F_NINF, r2 < k ? -m2 : F_NINF));
-        /* twice a value's error and its sum with the bias */
-        float tol = 0x1p-20f + 0x1p-21f * (fabsf(thr) + bmax);
-        if (KIND == APUS_SCORE_SQRTSOFTPLUS) tol = thr - bmax < 0.25f ? 0x1p-10f : tol + 0x1p-19f;
-        thr = fmaxf(thr - tol, -3.402823466e38f);                 /* masked ones never */
+        /* Twice the error of value v = p + bias and of the sum's rounding. The constant part holds
+         * for scores up to 1; those of sqrt-softplus have no upper end, and p <= |v| + bmax */
+        const bool small = thr - bmax < 0.25f;
+        auto tol = [&](float v) {
+            if (KIND == APUS_SCORE_SQRTSOFTPLUS) return small ? 0x1p-10f : 0x1p-18f + 0x1p-20f * (fabsf(v) + bmax);
+            return 0x1p-20f + 0x1p-21f * (fabsf(v) + bmax);
+        };
+        thr = fmaxf(thr - tol(thr), -3.402823466e38f);            /* masked ones never */
         thr = active ? thr : __builtin_inff();
         int cnt = 0;
 #pragma unroll
@@ -717,7 +721,7 @@ __global__ __launch_bounds__(256) void apus_route_row_kernel(ApusRouteArgs a, in
         wave_lds_order();                                         /* of equal ones a slot stays NaN */
         const float sv = w->best[lane].x, next = w->best[min(lane + 1, 63)].x;
         const bool last = l == k - 1 && n == k;                   /* none left that could be chosen */
-        const bool apart = sv - next > tol || (last && sv == sv);
+        const bool apart = sv - next > tol(sv) || (last && sv == sv);
         if (__any(l < k && !apart && !whole)) {
             double inv = inv_sum;
             if (SOFTMAX && !sum_all && a.bias) inv = exact_inv(); /* beside a bias the sum counts */
