@@ -682,10 +682,11 @@ __global__ __launch_bounds__(256) void apus_route_row_kernel(ApusRouteArgs a, in
         });
         float thr = -row_max(fmaxf(r1 < k ? -m1 : F_NINF, r2 < k ? -m2 : F_NINF));
         /* Twice the error of value v = p + bias and of the sum's rounding. The constant part holds
-         * for scores up to 1; those of sqrt-softplus have no upper end, and p <= |v| + bmax */
-        const bool small = thr - bmax < 0.25f;
+         * for scores up to 1; those of sqrt-softplus have no upper end, and p <= |v| + bmax. Its
+         * scores that decide may be small where the k-th value does not say otherwise */
+        const float least = KIND == APUS_SCORE_SQRTSOFTPLUS ? (thr - bmax < 0.25f ? 0x1p-10f : 0x1p-18f) : 0.0f;
         auto tol = [&](float v) {
-            if (KIND == APUS_SCORE_SQRTSOFTPLUS) return small ? 0x1p-10f : 0x1p-18f + 0x1p-20f * (fabsf(v) + bmax);
+            if (KIND == APUS_SCORE_SQRTSOFTPLUS) return least + 0x1p-20f * (fabsf(v) + bmax);
             return 0x1p-20f + 0x1p-21f * (fabsf(v) + bmax);
         };
         thr = fmaxf(thr - tol(thr), -3.402823466e38f);            /* masked ones never */

@@ -22,3 +22,23 @@ def test_route_large_scores_beside_small_ones(hip, rng, E, k, large, fine):
     np.put_along_axis(z, at, near, axis=1)
     bias = (fine * np.sqrt(large) * rng.standard_normal(E)).astype(np.float32) if fine else None
     check(hip, "softplus", z, bias, k, least=0.5)
+
+
+@pytest.mark.parametrize("E,k", [(64, 8), (256, 6), (320, 8), (64, 12)])
+@pytest.mark.parametrize("power", [14, 15, 17])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_route_biases_that_swamp_small_scores(hip, rng, E, k, power, sign):
+    """sums in which one step of fp32 is wider than the error of the scores. k experts have a
+    bias one step above the others' and a score just over half a step, k more a score just over
+    one and a half: less by 64-bit values, but a softplus near zero is known to 2^-24 only, and
+    fp32 sums of the former may come out a step below the latter's."""
+    s, step = 300, 2.0 ** (power - 23)
+    half = step * step / 4                        # the softplus of a score of half a step
+    kind = rng.permutation(np.minimum(np.arange(E) // k, 2))
+    a = half + 2.0 ** -23 * (0.30 + 0.15 * rng.random((s, E)))
+    b = 9 * half + 2.0 ** -23 * (0.55 + 0.10 * rng.random((s, E)))
+    z = np.where(kind == 2, -40.0, np.log(np.expm1(np.where(kind == 0, a, b))))
+    bias = (sign * 1.5 * 2.0 ** power + step * (kind == 0)).astype(np.float32)
+    # the former's scores may lie closer together than 2^-40 of the sums: their set is sure
+    idx, _ = check(hip, "softplus", z, bias, k, least=-1.0)
+    assert (kind[idx] == 0).all()
