@@ -633,15 +633,19 @@ __global__ __launch_bounds__(256) void apus_route_row_kernel(ApusRouteArgs a, in
         if (a.groups > 1 && a.keep < a.groups) {
             float g1 = m1, g2 = m2;
             top2_lanes(g1, g2, lpg);
-            const float mine = a.group_top == 2 && g2 > F_NINF ? g1 + g2 : g1;
+            const bool two = a.group_top == 2 && g2 > F_NINF;
+            const float mine = two ? g1 + g2 : g1, mag = two ? fabsf(g1) + fabsf(g2) : fabsf(g1);
             int above = 0;                                        /* lpg times the groups above */
             each_ror([&](auto c) { above += ror<decltype(c)::value>(mine) > mine ? 1 : 0; });
             active = above < a.keep * lpg;
-            const float lo = -row_max(active ? -mine : F_NINF), hi = row_max(active ? F_NINF : mine);
+            /* a group's error: that of its values (as for tol below; the smaller one may be small
+             * where the sum is not) and the roundings of three sums */
+            float err = 0x1p-19f + 0x1p-21f * (mag + 2.0f * bmax);
+            if (KIND == APUS_SCORE_SQRTSOFTPLUS && (two ? g2 : g1) - bmax < 0.25f) err += 0x1p-10f;
+            err = fminf(err, 3.402823466e38f);                    /* a sum of -inf stays that */
+            const float lo = -row_max(active ? err - mine : F_NINF), hi = row_max(active ? F_NINF : mine + err);
             const int kept = __popc((uint32_t)(__ballot(active) >> (lane & 48)) & 0xffffu);
-            /* sums of two values of 2^-20 error (small ones of sqrt-softplus: 2^-12) */
-            bool border = kept != a.keep * lpg || !(lo - hi > 0x1p-18f + 0x1p-20f * (fabsf(lo) + 2.0f * bmax));
-            if (KIND == APUS_SCORE_SQRTSOFTPLUS) border |= lo - 2.0f * bmax < 0.5f && !(lo - hi > 0x1p-9f);
+            const bool border = kept != a.keep * lpg || !(lo > hi);
             if (__any(border)) {                                  /* the groups by 64-bit values */
                 const double NINF = -__builtin_inf(), inv = SOFTMAX && !sum_all && a.bias ? exact_inv() : inv_sum;
                 double d1 = NINF, d2 = NINF;

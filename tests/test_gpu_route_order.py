@@ -42,3 +42,21 @@ def test_route_biases_that_swamp_small_scores(hip, rng, E, k, power, sign):
     # the former's scores may lie closer together than 2^-40 of the sums: their set is sure
     idx, _ = check(hip, "softplus", z, bias, k, least=-1.0)
     assert (kind[idx] == 0).all()
+
+
+@pytest.mark.parametrize("E,groups,keep,k", [(64, 8, 4, 4), (256, 8, 3, 6), (256, 4, 2, 2), (512, 8, 4, 8), (60, 5, 2, 2)])
+@pytest.mark.parametrize("first", [0.8, 1.5])
+@pytest.mark.parametrize("with_bias", [False, True])
+def test_route_groups_with_a_tiny_second_value(hip, rng, E, groups, keep, k, first, with_bias):
+    """a group's second value may be tiny where its sum is not: a softplus of 0.45 or 0.55 steps
+    of 2^-23 comes out as 0 or a whole one, and the groups' largest scores make up for that
+    difference in fp32 but not in 64 bits"""
+    s, per = 300, E // groups
+    low = rng.random((s, groups)) < 0.5
+    p1 = first + np.where(low, 1e-4, 0.0) + 1e-6 * rng.random((s, groups))
+    second = 2.0 ** -23 * np.where(low, 0.45, 0.55)
+    z = np.full((s, groups, per), -30.0) + rng.random((s, groups, per))
+    z[:, :, 1] = np.log(np.expm1(p1 * p1))
+    z[:, :, per - 1] = np.log(np.expm1(second))
+    bias = np.full(E, 0.125, np.float32) if with_bias else None
+    check(hip, "softplus", z.reshape(s, E), bias, k, groups, keep, 2, least=0.5)
