@@ -31,6 +31,13 @@ namespace {
 
 constexpr float F_NINF = -__builtin_inff();
 
+/* A score's error goes by the score. Known of it in value v = p + bias is p <= |v| + the largest
+ * |bias|: good where all biases are small, but one expert switched off by a bias of -1e9 would
+ * leave every token undecided (8192 x 256, sigmoid: 31.6 us for 7.9). Sigmoid and softmax end at 1;
+ * with a bias beyond this sqrt-softplus takes the largest score of the row too, which costs a
+ * reduction a token. */
+constexpr float APUS_LARGE_BIAS = 16.0f;
+
 /* logit as it is read: NaN masks like -inf, +inf is the largest number */
 __device__ __forceinline__ float logit_of(float z) { return z != z ? F_NINF : fminf(z, 3.402823466e38f); }
 
@@ -272,6 +279,10 @@ __global__ __launch_bounds__(256) void apus_route_kernel(ApusRouteArgs a, int lp
         }
     }
     bmax = apus_wave_max_dpp(bmax);
+    /* the largest score that value v = p + bias may hold: |v| + bmax, which bounds it best where
+     * the biases are small, and `top` */
+    float top = 1.0f;
+    auto reach = [&](float v, int n) { return fminf(v + n * bmax, n * top); };
     const bool sum_all = SOFTMAX && !a.renorm;
     const size_t step = (size_t)gridDim.x * 4 * tpw;
     for (; t0 < (size_t)a.s; t0 += step) {
@@ -337,6 +348,15 @@ __global__ __launch_bounds__(256) void apus_route_kernel(ApusRouteArgs a, int lp
                             if (has(i)) apus_gst<float>(sc + id(i), p[i]);
                     }
                 }
+                if constexpr (KIND == APUS_SCORE_SQRTSOFTPLUS) {
+                    top = __builtin_inff();
+                    if (bmax > APUS_LARGE_BIAS) {
+                        top = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < NE; ++i) top = fmaxf(top, p[i]);
+                        top = apus_wave_max_dpp(top);
+                    }
+                }
 #pragma unroll
                 for (int i = 0; i < NE; ++i) v[i] = z[i] > F_NINF ? p[i] + bias[i] : F_NINF;
             }
@@ -351,22 +371,22 @@ __global__ __launch_bounds__(256) void apus_route_kernel(ApusRouteArgs a, int lp
             if (a.groups > 1) {
                 float g1 = m1, g2 = m2;
                 top2_lanes(g1, g2, lpg);
-                const float mine = a.group_top == 2 && g2 > F_NINF ? g1 + g2 : g1;
+                const bool two = a.group_top == 2 && g2 > F_NINF;
+                const float mine = two ? g1 + g2 : g1, mag = two ? fabsf(g1) + fabsf(g2) : fabsf(g1);
                 int rank = 0;
                 for (int g = 0; g < a.groups; ++g) {
                     const float o = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, mine), g * lpg));
                     rank += o > mine ? 1 : 0;
                 }
-                /* the worst group kept and the best one left out; without them (equal scores)
-                 * or too close, the choice is not sure */
+                /* the worst group kept less its error and the best one left out with its own;
+                 * where they meet, or fewer or more than `keep` are kept (equal scores), the
+                 * choice is not sure */
                 if (a.keep < a.groups) {
-                    const uint64_t last = __ballot(active && rank == a.keep - 1), next = __ballot(active && rank == a.keep);
-                    border = !last || !next;
-                    if (!border) {
-                        const float lo = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, mine), __ffsll((unsigned long long)last) - 1));
-                        const float hi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, mine), __ffsll((unsigned long long)next) - 1));
-                        border = !(lo - hi > 0x1p-18f * (fabsf(lo) + 2.0f * bmax) + 1e-36f) || __popcll(last) != lpg;
-                    }
+                    const float err = fminf(0x1p-20f * reach(mag, 2) + 0x1p-22f * mag + 1e-36f, 3.402823466e38f);
+                    const bool in = active && rank < a.keep;
+                    const float lo = -apus_wave_max_dpp(in ? err - mine : F_NINF);
+                    const float hi = apus_wave_max_dpp(active && !in ? mine + err : F_NINF);
+                    border = __popcll(__ballot(in)) != a.keep * lpg || !(lo > hi);
                     active = active && rank < a.keep;
 #pragma unroll
                     for (int i = 0; i < NE; ++i) v[i] = active ? v[i] : F_NINF;
@@ -381,7 +401,7 @@ __global__ __launch_bounds__(256) void apus_route_kernel(ApusRouteArgs a, int lp
                 float r1 = m1, r2 = m2;
                 top2_lanes(r1, r2, of);
                 thr = -apus_wave_max_dpp(active ? -(k <= 8 ? r1 : r2) : F_NINF);
-                thr -= 0x1p-19f * (fabsf(thr) + bmax) + 1e-36f;
+                thr -= 0x1p-19f * reach(fabsf(thr), 1) + 0x1p-22f * fabsf(thr) + 1e-36f;
             }
             thr = fmaxf(thr, -3.402823466e38f);                   /* masked ones never */
             int n = 0;
@@ -416,7 +436,7 @@ __global__ __launch_bounds__(256) void apus_route_kernel(ApusRouteArgs a, int lp
                 wave_lds_order();
                 const float sv = w->best[lane].x, nx = w->best[min(lane + 1, 63)].x;
                 const bool last = lane == k - 1 && n == k;        /* none left that could be chosen */
-                const bool apart = sv - nx > 0x1p-19f * (fabsf(sv) + bmax) + 1e-36f || (last && sv == sv);
+                const bool apart = sv - nx > 0x1p-19f * reach(fabsf(sv), 1) + 0x1p-22f * fabsf(sv) + 1e-36f || (last && sv == sv);
                 if (__any(lane < k && !apart)) {
                     double inv = inv_sum, s = -__builtin_inf();
                     if (SOFTMAX && !sum_all && a.bias) inv = exact_inv();          /* beside a bias the sum counts */
@@ -517,13 +537,18 @@ __global__ __launch_bounds__(256) void apus_route_row_kernel(ApusRouteArgs a, in
     auto id = [&](int i) { return id0 + (V ? 4 * lpg * (i >> 2) + (i & 3) : lpg * i); };
     auto has = [&](int i) { return V ? i < ne : s0 + lpg * i < per; };
     const bool sum_all = SOFTMAX && !a.renorm, norm = SOFTMAX && (!a.renorm || a.bias || a.scores);
-    float *lbias = reinterpret_cast<float *>(lds + 4 * sizeof(RowLds) + 4 * E * sizeof(double)), bmax = 0.0f;
+    /* largest |bias| and largest bias of the finite ones */
+    float *lbias = reinterpret_cast<float *>(lds + 4 * sizeof(RowLds) + 4 * E * sizeof(double)), bmax = 0.0f, btop = 0.0f;
     if (a.bias) {
         for (int e = threadIdx.x; e < E; e += 256) lbias[e] = a.bias[e] == a.bias[e] ? a.bias[e] : F_NINF;
         __syncthreads();
         for (int e = lane; e < E; e += 64)
-            if (fabsf(lbias[e]) < __builtin_inff()) bmax = fmaxf(bmax, fabsf(lbias[e]));
+            if (fabsf(lbias[e]) < __builtin_inff()) {
+                bmax = fmaxf(bmax, fabsf(lbias[e]));
+                btop = fmaxf(btop, lbias[e]);
+            }
         bmax = apus_wave_max_dpp(bmax);
+        btop = apus_wave_max_dpp(btop);
     }
     const size_t step = (size_t)gridDim.x * 16;
     for (size_t t0 = ((size_t)blockIdx.x * 4 + wave) * 4; t0 < (size_t)a.s; t0 += step) {
@@ -607,6 +632,15 @@ __global__ __launch_bounds__(256) void apus_route_row_kernel(ApusRouteArgs a, in
                     if (has(i)) apus_gst<float>(sc + id(i), v[i]);
             }
         }
+        /* as above: the largest score that v = p + bias may hold (sqrt-softplus alone asks) */
+        float top = __builtin_inff();
+        if (KIND == APUS_SCORE_SQRTSOFTPLUS && bmax > APUS_LARGE_BIAS) {
+            top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NE; ++i) top = fmaxf(top, v[i]);
+            top = row_max(top);
+        }
+        auto reach = [&](float v, int n) { return fminf(v + n * bmax, n * top); };
         if (a.bias) {
             if constexpr (V) {
 #pragma unroll
@@ -640,8 +674,8 @@ __global__ __launch_bounds__(256) void apus_route_row_kernel(ApusRouteArgs a, in
             active = above < a.keep * lpg;
             /* a group's error: that of its values (as for tol below; the smaller one may be small
              * where the sum is not) and the roundings of three sums */
-            float err = 0x1p-19f + 0x1p-21f * (mag + 2.0f * bmax);
-            if (KIND == APUS_SCORE_SQRTSOFTPLUS && (two ? g2 : g1) - bmax < 0.25f) err += 0x1p-10f;
+            float err = 0x1p-19f + 0x1p-22f * mag;
+            if (KIND == APUS_SCORE_SQRTSOFTPLUS) err += 0x1p-21f * reach(mag, 2) + ((two ? g2 : g1) - btop < 0.25f ? 0x1p-10f : 0.0f);
             err = fminf(err, 3.402823466e38f);                    /* a sum of -inf stays that */
             const float lo = -row_max(active ? err - mine : F_NINF), hi = row_max(active ? F_NINF : mine + err);
             const int kept = __popc((uint32_t)(__ballot(active) >> (lane & 48)) & 0xffffu);
@@ -686,12 +720,12 @@ __global__ __launch_bounds__(256) void apus_route_row_kernel(ApusRouteArgs a, in
         });
         float thr = -row_max(fmaxf(r1 < k ? -m1 : F_NINF, r2 < k ? -m2 : F_NINF));
         /* Twice the error of value v = p + bias and of the sum's rounding. The constant part holds
-         * for scores up to 1; those of sqrt-softplus have no upper end, and p <= |v| + bmax. Its
-         * scores that decide may be small where the k-th value does not say otherwise */
-        const float least = KIND == APUS_SCORE_SQRTSOFTPLUS ? (thr - bmax < 0.25f ? 0x1p-10f : 0x1p-18f) : 0.0f;
+         * for scores up to 1; those of sqrt-softplus have no upper end. Its scores that decide
+         * may be small (p = v - bias) where the k-th value does not say otherwise */
+        const float least = KIND == APUS_SCORE_SQRTSOFTPLUS ? (thr - btop < 0.25f ? 0x1p-10f : 0x1p-18f) : 0x1p-20f;
         auto tol = [&](float v) {
-            if (KIND == APUS_SCORE_SQRTSOFTPLUS) return least + 0x1p-20f * (fabsf(v) + bmax);
-            return 0x1p-20f + 0x1p-21f * (fabsf(v) + bmax);
+            const float t = least + 0x1p-22f * fabsf(v);
+            return KIND == APUS_SCORE_SQRTSOFTPLUS ? t + 0x1p-20f * reach(fabsf(v), 1) : t;
         };
         thr = fmaxf(thr - tol(thr), -3.402823466e38f);            /* masked ones never */
         thr = active ? thr : __builtin_inff();

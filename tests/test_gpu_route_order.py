@@ -1,10 +1,12 @@
 """The order of apus_hip_route_dev where fp32 scores of very different size meet: large
 scores beside ordinary ones, biases that swamp the scores, groups whose second value is tiny.
 The choice has to be that of the 64-bit values (tests/test_gpu_route.py says what is compared)."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
-from test_gpu_route import check
+from test_gpu_route import KINDS, check
 
 pytestmark = pytest.mark.gpu
 
@@ -60,3 +62,49 @@ def test_route_groups_with_a_tiny_second_value(hip, rng, E, groups, keep, k, fir
     z[:, :, per - 1] = np.log(np.expm1(second))
     bias = np.full(E, 0.125, np.float32) if with_bias else None
     check(hip, "softplus", z.reshape(s, E), bias, k, groups, keep, 2, least=0.5)
+
+
+SHAPES = [(256, 8, 1, 1), (256, 8, 8, 4), (320, 8, 1, 1), (512, 8, 2, 1), (64, 12, 1, 1), (64, 6, 16, 7)]
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("E,k,groups,keep", SHAPES)
+@pytest.mark.parametrize("large", [-1e9, -1e4, 1e4, 1e9, 3.4e38])
+@pytest.mark.parametrize("top", [1, 2])
+def test_route_some_large_biases(hip, rng, kind, E, k, groups, keep, large, top):
+    """experts, a pair in one group or a whole group moved far off by their bias; close scores"""
+    z = np.round(16 * (1.5 * rng.standard_normal((60, E)))) / 16 + 2.0 ** -20 * rng.integers(0, 3, (60, E))
+    bias = (0.05 * rng.standard_normal(E)).astype(np.float32)
+    bias[[1, E // 2]] = large
+    check(hip, kind, z, bias, k, groups, keep, top, least=0.2)
+    bias[:E // 8] = large
+    bias[E - 3] = -large
+    check(hip, kind, z, bias, k, groups, keep, top, least=-1.0)
+
+
+def time_us(hip, kind, z, bias, k, groups, keep):
+    s, E = z.shape
+    L = hip.lib()
+    dz, db, di, dw = hip.DevBuf.from_array(z), hip.DevBuf.from_array(bias), hip.DevBuf(s * k * 4), hip.DevBuf(s * k * 4)
+    cfg = hip.ApusHipRoute(KINDS[kind], k, groups, keep, 2, 1, 2.5)
+    times = []
+    for _ in range(7):
+        hip.synchronize()
+        L.apus_hip_timer_start()
+        for _ in range(20):
+            hip._check(L.apus_hip_route_dev(C.byref(cfg), dz.ptr, db.ptr, s, E, di.ptr, dw.ptr, None), "route")
+        times.append(L.apus_hip_timer_stop() / 20 * 1e3)
+    return sorted(times)[3]
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("E,k,groups,keep", SHAPES[:5])
+def test_route_a_large_bias_costs_little(hip, rng, kind, E, k, groups, keep):
+    """an expert switched off by -1e9 or by -inf: about the same time (1.9 to 4.2 times
+    where every token is ranked in 64 bits)"""
+    z = (1.5 * rng.standard_normal((8192, E))).astype(np.float32)
+    bias = (0.05 * rng.standard_normal(E)).astype(np.float32)
+    off = bias.copy()
+    bias[5], off[5] = -np.inf, -1e9
+    a, b = (time_us(hip, kind, z, v, k, groups, keep) for v in (bias, off))
+    assert b < 1.6 * a, (a, b)
