@@ -8,6 +8,7 @@
 #include "apus_internal.h"
 
 #include <algorithm>
+#include <type_traits>
 
 typedef int apus_v4i __attribute__((ext_vector_type(4)));
 /* the vector unit takes 8- and 16-byte accesses at any address (2997 x 18270 x 112, BF16 rows of
@@ -312,18 +313,27 @@ __global__ __launch_bounds__(64 * B::NW) void apus_i8_block_kernel(ApusI8Args a)
     }
 }
 
+/* Kernel's limit of dynamic LDS raised to LDS bytes, once. The kernel is a template argument: kernels
+ * of one type passed as values would share the static, and only the first would be raised */
+template <auto Kernel, int LDS>
+hipError_t apus_i8_lds_limit() {
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(Kernel),
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    return attr;
+}
+
 template <class B>
 hipError_t apus_launch_i8_block(const ApusI8Args &a, hipStream_t st) {
-    auto go = [&](auto kernel) {
-        static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
-                                                           hipFuncAttributeMaxDynamicSharedMemorySize, B::LDS);
+    auto go = [&](auto yb) {
+        constexpr auto kernel = &apus_i8_block_kernel<B, decltype(yb)::value>;
+        const hipError_t attr = apus_i8_lds_limit<kernel, B::LDS>();
         if (attr != hipSuccess) return attr;
         const size_t tiles = ((size_t)a.M + B::BM - 1) / B::BM * (((size_t)a.O + B::BN - 1) / B::BN);
         if (tiles > 0xffffffffu / (64 * B::NW)) return hipErrorInvalidValue;
         hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(64 * B::NW), B::LDS, st, a);
         return hipGetLastError();
     };
-    return a.y_bf16 ? go(&apus_i8_block_kernel<B, true>) : go(&apus_i8_block_kernel<B, false>);
+    return a.y_bf16 ? go(std::true_type{}) : go(std::false_type{});
 }
 
 /*
@@ -441,16 +451,16 @@ hipError_t apus_launch_i8_narrow(const ApusI8Args &a, hipStream_t st) {
     constexpr int ring = NW * PD * ((HALF ? 1 : 2 * TM) + 2 * TN) * 1024, sums = NW * TM * TN * 1024;
     constexpr int lds = ring > sums ? ring : sums;
     static_assert(lds <= 160 * 1024, "LDS");
-    auto go = [&](auto kernel) {
-        static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
-                                                           hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    auto go = [&](auto yb) {
+        constexpr auto kernel = &apus_i8_narrow_kernel<TM, TN, NW, PD, HALF, decltype(yb)::value>;
+        const hipError_t attr = apus_i8_lds_limit<kernel, lds>();
         if (attr != hipSuccess) return attr;
         const size_t wgs = ((size_t)a.O + 16 * TN - 1) / (16 * TN) * (((size_t)a.M + 16 * TM - 1) / (16 * TM));
         if (wgs > 0xffffffffu / (64 * NW)) return hipErrorInvalidValue;
         hipLaunchKernelGGL(kernel, dim3((unsigned)wgs), dim3(64 * NW), lds, st, a);
         return hipGetLastError();
     };
-    return a.y_bf16 ? go(&apus_i8_narrow_kernel<TM, TN, NW, PD, HALF, true>) : go(&apus_i8_narrow_kernel<TM, TN, NW, PD, HALF, false>);
+    return a.y_bf16 ? go(std::true_type{}) : go(std::false_type{});
 }
 
 /*
