@@ -389,8 +389,9 @@ __global__ __launch_bounds__(256) void apus_i8_quant_any_kernel(const void *__re
                                                                 float *__restrict__ scales) {
     const int tid = threadIdx.x;
     __shared__ unsigned red[4];
-    for (int row = blockIdx.x; row < M; row += gridDim.x) {
-        const size_t off = (size_t)row * K;
+    /* 64 bits: up to ROWS_MAX rows further, an int may pass its end */
+    for (size_t row = blockIdx.x; row < (size_t)M; row += gridDim.x) {
+        const size_t off = row * K;
         unsigned m = 0;
         for (int k = tid; k < K; k += 256)
             m = max(m, apus_f2u(apus_bf16_rne(ld_elem<XB>(x, off + k))) & 0x7fffffffu);
