@@ -197,6 +197,7 @@ SIGNATURES = {
     "apus_hip_host_bf16_round": (C.c_float, [C.c_float]),
     "apus_hip_host_e4m3_quant": (C.c_uint8, [C.c_float]),
     "apus_hip_host_act_scale": (C.c_float, [C.c_float]),
+    "apus_hip_host_i8_schedule": (None, [C.c_int, C.c_int, C.c_int, C.POINTER(C.c_int32)]),
 }
 
 _lib = None

@@ -2273,5 +2273,9 @@ int apus_hip_check_e4m3_hw(unsigned *mismatches, unsigned *last_bad_bits) {
 float apus_hip_host_bf16_round(float x) { return apus_bf16_rne(x); }
 uint8_t apus_hip_host_e4m3_quant(float x) { return (uint8_t)apus_e4m3_code(x); }
 float apus_hip_host_act_scale(float amax) { return apus_pow2_from_exp(apus_act_scale_exp(amax)); }
+void apus_hip_host_i8_schedule(int M, int O, int K, int32_t shape[5]) {
+    const ApusI8Shape s = apus_i8_schedule(M, O, K);
+    shape[0] = s.rows; shape[1] = s.cols; shape[2] = s.split; shape[3] = s.depth; shape[4] = s.threads;
+}
 
 }  // extern "C"

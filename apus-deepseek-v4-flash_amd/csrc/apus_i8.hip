@@ -571,73 +571,118 @@ hipError_t apus_launch_i8_gemv(const ApusI8Args &a, hipStream_t st) {
     return a.y_bf16 ? go(&apus_i8_gemv_kernel<R, U, XS, true>) : go(&apus_i8_gemv_kernel<R, U, XS, false>);
 }
 
+namespace {
+
+/* a launch holds fewer than 2^32 threads */
+constexpr size_t THREADS_MAX = 0xffffffffu;
+
 /* Rows and chunks a wave: about 4 KB of weights under way in each, from as many rows as
  * that takes (us, 1 x 4 / 2 x 2 / 4 x 1: K 8192, 4096 channels 7.1 / 7.6 / 8.8; K 4096, 1024
  * channels 2.8 / 3.4 / 4.5, 129280 74 / 75 / 79 (7.1 TB/s); K 2048, 4096 channels 3.8 / 3.4 /
  * 3.7; K 1024, 32768 channels 12.5 / 8.0 / 7.0; more of a row or more rows at once are
  * slower everywhere). Bound by HBM, or by the launch and one pass of latency. */
+int gemv_rows(int K) { return K > 2048 ? 1 : K > 1024 ? 2 : 4; }
+/* whether the one-row schedule's grid holds O channels */
+bool gemv_fits(int O, int K) {
+    return O <= 1 << 26 && ((size_t)O + 4 * gemv_rows(K) - 1) / (4 * gemv_rows(K)) <= THREADS_MAX / 256;
+}
+
+}  // namespace
+
 template <int XS>
 hipError_t apus_launch_i8_gemv_x(const ApusI8Args &a, hipStream_t st) {
-    return a.K > 2048 ? apus_launch_i8_gemv<1, 4, XS>(a, st) : a.K > 1024 ? apus_launch_i8_gemv<2, 2, XS>(a, st)
-                                                                          : apus_launch_i8_gemv<4, 1, XS>(a, st);
+    const int rows = gemv_rows(a.K);
+    return rows == 1 ? apus_launch_i8_gemv<1, 4, XS>(a, st) : rows == 2 ? apus_launch_i8_gemv<2, 2, XS>(a, st)
+                                                                        : apus_launch_i8_gemv<4, 1, XS>(a, st);
+}
+
+namespace {
+
+struct Sched {
+    hipError_t (*launch)(const ApusI8Args &, hipStream_t);
+    ApusI8Shape shape;
+    float c, e, t, c2, e2;                /* the modelled time, in us */
+};
+template <int TM, int TN, int NW, int PD, bool HALF>
+constexpr Sched narrow_sched(float c, float e, float t, float c2, float e2) {
+    return {apus_launch_i8_narrow<TM, TN, NW, PD, HALF>, {HALF ? 8 : 16 * TM, 16 * TN, NW, PD, 64 * NW}, c, e, t, c2, e2};
+}
+template <class B>
+constexpr Sched block_sched(float c, float e, float t, float c2, float e2) {
+    return {apus_launch_i8_block<B>, {B::BM, B::BN, 1, B::NST, 64 * B::NW}, c, e, t, c2, e2};
+}
+constexpr Sched FEW[] = {narrow_sched<1, 1, 4, 4, true>(0, 0, 0, 0, 0), narrow_sched<1, 2, 2, 4, true>(0, 0, 0, 0, 0)};
+/* Fitted to every other of 228 measured shapes (9 to 4096 rows, 256 to 32768 channels, K 512
+ * to 8192; mean error 6 to 11 % a schedule); on the rest the choice is 0.7 % behind the
+ * fastest of all in the geometric mean, 12 % at worst. Without 256 x 128 it is 0.8 %, 23 % at
+ * worst; without any other, 1.0 to 8.2 %. */
+constexpr Sched MORE[] = {
+    narrow_sched<1, 1, 4, 4, false>(0.046f, 1.04f, 1.46f, 0.105f, 0.99f),
+    narrow_sched<2, 2, 2, 4, false>(0.129f, 0.54f, 2.31f, 0.0f, 0.0f),
+    narrow_sched<4, 2, 4, 2, false>(0.159f, 2.23f, 0.81f, 0.0f, 0.0f),
+    block_sched<ApusI8Blk<64, 64, 4, 2, 4>>(0.216f, 1.00f, 2.48f, 0.419f, 2.42f),
+    block_sched<ApusI8Blk<64, 128, 2, 4, 4>>(0.352f, 3.24f, 0.55f, 0.0f, 0.0f),
+    block_sched<ApusI8Blk<128, 128, 2, 4, 4>>(0.481f, 5.69f, -1.01f, 0.0f, 0.0f),
+    block_sched<ApusI8Blk<128, 128, 2, 4, 2>>(0.779f, 0.12f, 3.03f, 1.020f, 4.95f),
+    block_sched<ApusI8Blk<256, 128, 4, 2, 3>>(0.797f, 7.71f, -0.71f, 0.0f, 0.0f),
+    block_sched<ApusI8Blk<256, 256, 2, 4, 2>>(1.403f, 13.47f, -3.17f, 0.0f, 0.0f),
+};
+
+size_t tiles_of(const ApusI8Shape &s, int M, int O) { return ((size_t)M + s.rows - 1) / s.rows * (((size_t)O + s.cols - 1) / s.cols); }
+
+/* The schedule of 2 rows and more with 16-byte pieces; null where no grid holds the tiles. */
+const Sched *choose(int M, int O, int K) {
+    if (O > 1 << 26) return nullptr;
+    if (M <= 8)
+        /* Short rows of many channels: twice the channels a workgroup and half the waves
+         * (16 x 4 / 32 x 2, 8 rows, us: K 1024, 8192 / 16384 / 32768 channels 3.7 / 6.5 / 10.0
+         * against 3.8 / 5.9 / 8.5; K 2048, 12288 channels 6.8 against 7.6; K 4096, 32768 25.8
+         * against 28.6; 4096 x 8192 8.0 against 10.5) */
+        return &FEW[K <= 1024 && O > 8192];
+    /* More rows: the schedule whose modelled time is least. n workgroups of `steps`
+     * steps of 128 bytes of K take, in us, rounds of 256 CUs times (c steps + e); where
+     * two workgroups fit a CU, rounds of 512 times (c2 steps + e2), a last one of up to
+     * 256 the former; + t. */
+    const float steps = (float)((K + 127) / 128);
+    const Sched *best = nullptr;
+    float least = 0.0f;
+    for (const Sched &c : MORE) {
+        const size_t n = tiles_of(c.shape, M, O), left = n % 512;
+        if (n > THREADS_MAX / c.shape.threads) continue;
+        const float one = c.c * steps + c.e, two = c.c2 * steps + c.e2;
+        const float us = c.c2 == 0.0f ? (float)((n + 255) / 256) * one + c.t
+                                      : (float)(n / 512) * two + (left == 0 ? 0.0f : left <= 256 ? one : two) + c.t;
+        if (!best || us < least) {
+            best = &c;
+            least = us;
+        }
+    }
+    return best;
+}
+
+}  // namespace
+
+ApusI8Shape apus_i8_schedule(int M, int O, int K) {
+    if (M == 1) return gemv_fits(O, K) ? ApusI8Shape{1, 4 * gemv_rows(K), 1, 1, 256} : ApusI8Shape{};
+    const Sched *s = choose(M, O, K);
+    return s ? s->shape : ApusI8Shape{};
 }
 
 /* one row, fp32 or BF16 in: quantised inside the product's launch */
 bool apus_i8_fused_ok(const ApusI8Args *a) {
-    return a->M == 1 && a->O <= 1 << 26 && a->K % 16 == 0 && a->K <= 32768 && (((uintptr_t)a->x | (uintptr_t)a->w) & 15) == 0;
+    return a->M == 1 && gemv_fits(a->O, a->K) && a->K % 16 == 0 && a->K <= 32768 && (((uintptr_t)a->x | (uintptr_t)a->w) & 15) == 0;
 }
 
 hipError_t apus_launch_i8_gemm(const ApusI8Args *a, hipStream_t st) {
     if (a->M <= 0) return hipSuccess;
     if (a->x) return a->x_bf16 ? apus_launch_i8_gemv_x<2>(*a, st) : apus_launch_i8_gemv_x<1>(*a, st);
-    /* (more channels than the one-row schedule has workgroups for: the loops of the last kernel) */
-    if (a->K % 16 == 0 && (((uintptr_t)a->a | (uintptr_t)a->w) & 15) == 0 && a->O <= 1 << 26) {
-        if (a->M == 1) return apus_launch_i8_gemv_x<0>(*a, st);
-        if (a->M <= 8)
-            /* Short rows of many channels: twice the channels a workgroup and half the waves
-             * (16 x 4 / 32 x 2, 8 rows, us: K 1024, 8192 / 16384 / 32768 channels 3.7 / 6.5 / 10.0
-             * against 3.8 / 5.9 / 8.5; K 2048, 12288 channels 6.8 against 7.6; K 4096, 32768 25.8
-             * against 28.6; 4096 x 8192 8.0 against 10.5) */
-            return a->K <= 1024 && a->O > 8192 ? apus_launch_i8_narrow<1, 2, 2, 4, true>(*a, st)
-                                               : apus_launch_i8_narrow<1, 1, 4, 4, true>(*a, st);
-        /* More rows: the schedule whose modelled time is least. n workgroups of `steps`
-         * steps of 128 bytes of K take, in us, rounds of 256 CUs times (c steps + e); where
-         * two workgroups fit a CU, rounds of 512 times (c2 steps + e2), a last one of up to
-         * 256 the former; + t. Fitted to every other of 228 measured shapes (9 to 4096 rows,
-         * 256 to 32768 channels, K 512 to 8192; mean error 6 to 11 % a schedule); on the
-         * rest the choice is 0.7 % behind the fastest of all in the geometric mean, 12 % at
-         * worst. Without 256 x 128 it is 0.8 %, 23 % at worst; without any other, 1.0 to 8.2 %. */
-        static const struct {
-            hipError_t (*launch)(const ApusI8Args &, hipStream_t);
-            int bm, bn;
-            float c, e, t, c2, e2;
-        } sched[] = {
-            {apus_launch_i8_narrow<1, 1, 4, 4, false>, 16, 16, 0.046f, 1.04f, 1.46f, 0.105f, 0.99f},
-            {apus_launch_i8_narrow<2, 2, 2, 4, false>, 32, 32, 0.129f, 0.54f, 2.31f, 0.0f, 0.0f},
-            {apus_launch_i8_narrow<4, 2, 4, 2, false>, 64, 32, 0.159f, 2.23f, 0.81f, 0.0f, 0.0f},
-            {apus_launch_i8_block<ApusI8Blk<64, 64, 4, 2, 4>>, 64, 64, 0.216f, 1.00f, 2.48f, 0.419f, 2.42f},
-            {apus_launch_i8_block<ApusI8Blk<64, 128, 2, 4, 4>>, 64, 128, 0.352f, 3.24f, 0.55f, 0.0f, 0.0f},
-            {apus_launch_i8_block<ApusI8Blk<128, 128, 2, 4, 4>>, 128, 128, 0.481f, 5.69f, -1.01f, 0.0f, 0.0f},
-            {apus_launch_i8_block<ApusI8Blk<128, 128, 2, 4, 2>>, 128, 128, 0.779f, 0.12f, 3.03f, 1.020f, 4.95f},
-            {apus_launch_i8_block<ApusI8Blk<256, 128, 4, 2, 3>>, 256, 128, 0.797f, 7.71f, -0.71f, 0.0f, 0.0f},
-            {apus_launch_i8_block<ApusI8Blk<256, 256, 2, 4, 2>>, 256, 256, 1.403f, 13.47f, -3.17f, 0.0f, 0.0f},
-        };
-        const float steps = (float)((a->K + 127) / 128);
-        int best = 0;
-        float least = 0.0f;
-        for (int i = 0; i < (int)(sizeof sched / sizeof *sched); ++i) {
-            const auto &c = sched[i];
-            const size_t n = ((size_t)a->M + c.bm - 1) / c.bm * (((size_t)a->O + c.bn - 1) / c.bn);
-            const float one = c.c * steps + c.e, two = c.c2 * steps + c.e2;
-            const size_t left = n % 512;
-            const float us = c.c2 == 0.0f ? (float)((n + 255) / 256) * one + c.t
-                                          : (float)(n / 512) * two + (left == 0 ? 0.0f : left <= 256 ? one : two) + c.t;
-            if (i == 0 || us < least) {
-                best = i;
-                least = us;
-            }
+    if (a->K % 16 == 0 && (((uintptr_t)a->a | (uintptr_t)a->w) & 15) == 0) {
+        if (a->M == 1) {
+            if (gemv_fits(a->O, a->K)) return apus_launch_i8_gemv_x<0>(*a, st);
+        } else if (const Sched *s = choose(a->M, a->O, a->K)) {
+            return s->launch(*a, st);
         }
-        return sched[best].launch(*a, st);
+        /* more channels or tiles than a launch has workgroups for: the loops of the last kernel */
     }
     const size_t tiles = ((size_t)a->M + 63) / 64 * (((size_t)a->O + 63) / 64);
     auto go = [&](auto kernel) {

@@ -350,5 +350,12 @@ typedef struct {
 /* whether the product takes a->x itself, without apus_launch_i8_quant before it */
 bool apus_i8_fused_ok(const ApusI8Args *a);
 hipError_t apus_launch_i8_gemm(const ApusI8Args *a, hipStream_t st);
+/* the tile that the product takes for a shape with K % 16 == 0 and 16-byte alignment: rows and
+ * channels of a workgroup, waves that split K, steps of 128 bytes of K under way, threads;
+ * zeros: the plain kernel */
+typedef struct {
+    int rows, cols, split, depth, threads;
+} ApusI8Shape;
+ApusI8Shape apus_i8_schedule(int M, int O, int K);
 
 #endif /* APUS_INTERNAL_H */

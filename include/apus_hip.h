@@ -575,6 +575,10 @@ int   apus_hip_check_e4m3_hw(unsigned *mismatches, unsigned *last_bad_bits);
 float    apus_hip_host_bf16_round(float x);
 uint8_t  apus_hip_host_e4m3_quant(float x);
 float    apus_hip_host_act_scale(float amax);
+/* The tile that apus_hip_i8_gemm_dev takes for a shape with K % 16 == 0 and 16-byte aligned
+ * codes (a test hook): rows and channels of a workgroup, waves that split K, steps of 128 bytes
+ * of K under way, threads; zeros for the plain kernel, whose workgroups loop over tiles. */
+void     apus_hip_host_i8_schedule(int M, int O, int K, int32_t shape[5]);
 
 #ifdef __cplusplus
 }
