@@ -139,9 +139,9 @@ template <int BM_, int BN_, int WM_, int WN_, int NST_>
 struct ApusI8Blk {
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NST = NST_, NW = WM * WN;
     static constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
-    static constexpr int LX = BM / 8, LT = (BM + BN) / 8, LPW = (LT + NW - 1) / NW;  /* loads: activations, all, a wave's */
+    static constexpr int LX = BM / 8, LT = (BM + BN) / 8, LPW = LT / NW;  /* loads: activations, all, a wave's */
     static constexpr int STB = (BM + BN) * 128, LDS = NST * STB + (BM + BN) * 4;  /* stages; scales */
-    static_assert(BM % (WM * 16) == 0 && BN % (WN * 16) == 0 && (BM + BN) % 64 == 0 && LDS <= 160 * 1024, "block shape");
+    static_assert(BM % (WM * 16) == 0 && BN % (WN * 16) == 0 && (BM + BN) % 64 == 0 && LT % NW == 0 && LDS <= 160 * 1024, "block shape");
 };
 
 template <class B, bool YB>
@@ -155,12 +155,11 @@ __global__ __launch_bounds__(64 * B::NW) void apus_i8_block_kernel(ApusI8Args a)
     apus_i8_tile(blockIdx.x, mt, nt, mb, nb);
     const int m0 = mb * B::BM, n0 = nb * B::BN, K = a.K, nq = (K + 127) >> 7, tail = K & 127;
     const unsigned lbase = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)lds);
-    /* a wave's loads (the last ones again where they do not divide evenly): a
-     * uniform base and 32-bit lane offsets; the last step's chunks past K read the
-     * row's last chunk */
+    /* a wave's loads: a uniform base and 32-bit lane offsets; the last step's chunks past K
+     * read the row's last chunk */
     const uint8_t *xb = (const uint8_t *)a.a + (size_t)m0 * K, *wb = (const uint8_t *)a.w + (size_t)n0 * K;
     unsigned off[B::LPW];
-    auto load_of = [&](int u) { return min(wave * B::LPW + u, B::LT - 1); };
+    auto load_of = [&](int u) { return wave * B::LPW + u; };
     /* the lane's chunk of row 8 j + lane / 8, j = load_of(u) or, of a weight, an even LX less */
     auto chunk_in = [&](int u) { return (lane & 7) ^ ((4 * load_of(u) + (lane >> 4)) & 7); };
 #pragma unroll
