@@ -12,8 +12,11 @@ product  apus_hip_i8_gemm_dev: 8-bit integer codes times 8-bit integer weights.
 linear   apus_hip_i8_linear_dev: fp32 activations in, quantised per token, product.
 
 run() gives the plain forms in elementary operations, or, where `own` is set,
-makes the calls. Codes come back as what they hold: E4M3 values or integers,
-with their scales beside them.
+makes the calls. Those run on the backend's stream, which knows nothing of
+torch's: what torch has under way is waited for before a state's first call, and
+the tensors that run() returns hold the results once the device, or the backend's
+stream (apus_hip.synchronize), has been waited for. Codes come back as what they
+hold: E4M3 values or integers, with their scales beside them.
 """
 import ctypes as C
 import math
@@ -259,6 +262,8 @@ def _call(st):
         sys.path.insert(0, _PKG)
     import apus_hip as H
     H.enable()
+    # inputs and zeroed outputs may still be under way on torch's stream
+    torch.cuda.synchronize()
     L, case, kind = H.lib(), st["case"], st["case"]["kind"]
     if kind == "norm":
         flags = (H.X_BF16 | H.Y_BF16 if case["bf16"] else 0) | (H.Q_I8 if case["quant"] == "i8" else 0)
