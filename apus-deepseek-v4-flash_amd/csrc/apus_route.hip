@@ -537,18 +537,21 @@ __global__ __launch_bounds__(256) void apus_route_row_kernel(ApusRouteArgs a, in
     auto id = [&](int i) { return id0 + (V ? 4 * lpg * (i >> 2) + (i & 3) : lpg * i); };
     auto has = [&](int i) { return V ? i < ne : s0 + lpg * i < per; };
     const bool sum_all = SOFTMAX && !a.renorm, norm = SOFTMAX && (!a.renorm || a.bias || a.scores);
-    /* largest |bias| and largest bias of the finite ones */
+    /* largest |bias| of the finite ones, and a bound of their largest: where |bias| is small the
+     * former will do */
     float *lbias = reinterpret_cast<float *>(lds + 4 * sizeof(RowLds) + 4 * E * sizeof(double)), bmax = 0.0f, btop = 0.0f;
     if (a.bias) {
         for (int e = threadIdx.x; e < E; e += 256) lbias[e] = a.bias[e] == a.bias[e] ? a.bias[e] : F_NINF;
         __syncthreads();
         for (int e = lane; e < E; e += 64)
-            if (fabsf(lbias[e]) < __builtin_inff()) {
-                bmax = fmaxf(bmax, fabsf(lbias[e]));
-                btop = fmaxf(btop, lbias[e]);
-            }
-        bmax = apus_wave_max_dpp(bmax);
-        btop = apus_wave_max_dpp(btop);
+            if (fabsf(lbias[e]) < __builtin_inff()) bmax = fmaxf(bmax, fabsf(lbias[e]));
+        btop = bmax = apus_wave_max_dpp(bmax);
+        if (KIND == APUS_SCORE_SQRTSOFTPLUS && bmax > APUS_LARGE_BIAS) {
+            btop = 0.0f;
+            for (int e = lane; e < E; e += 64)
+                if (lbias[e] < __builtin_inff()) btop = fmaxf(btop, lbias[e]);
+            btop = apus_wave_max_dpp(btop);
+        }
     }
     const size_t step = (size_t)gridDim.x * 16;
     for (size_t t0 = ((size_t)blockIdx.x * 4 + wave) * 4; t0 < (size_t)a.s; t0 += step) {
@@ -722,10 +725,10 @@ __global__ __launch_bounds__(256) void apus_route_row_kernel(ApusRouteArgs a, in
         /* Twice the error of value v = p + bias and of the sum's rounding. The constant part holds
          * for scores up to 1; those of sqrt-softplus have no upper end. Its scores that decide
          * may be small (p = v - bias) where the k-th value does not say otherwise */
-        const float least = KIND == APUS_SCORE_SQRTSOFTPLUS ? (thr - btop < 0.25f ? 0x1p-10f : 0x1p-18f) : 0x1p-20f;
+        const float least = KIND == APUS_SCORE_SQRTSOFTPLUS && thr - btop < 0.25f ? 0x1p-10f : 0x1p-20f;
         auto tol = [&](float v) {
             const float t = least + 0x1p-22f * fabsf(v);
-            return KIND == APUS_SCORE_SQRTSOFTPLUS ? t + 0x1p-20f * reach(fabsf(v), 1) : t;
+            return KIND == APUS_SCORE_SQRTSOFTPLUS ? t + 0x1.4p-21f * reach(fabsf(v), 1) : t;
         };
         thr = fmaxf(thr - tol(thr), -3.402823466e38f);            /* masked ones never */
         thr = active ? thr : __builtin_inff();
