@@ -556,7 +556,7 @@ __global__ __launch_bounds__(256) void apus_route_row_kernel(ApusRouteArgs a, in
     const size_t step = (size_t)gridDim.x * 16;
     for (size_t t0 = ((size_t)blockIdx.x * 4 + wave) * 4; t0 < (size_t)a.s; t0 += step) {
         /* worked out in each round: kept over all of them, the experts' numbers and addresses take 40
-         * registers (32768 tokens, sqrt-softplus 26.6 us so, 20.5 without, sigmoid and groups
+         * registers (32768 tokens, sqrt-softplus 26.6 us so, 20.6 without, sigmoid and groups
          * 23.6, 22.6; 64 tokens 6.1, 6.25). For a softmax in fours three waves a SIMD have
          * room for them (15.7, 16.1) */
         if constexpr (!(SOFTMAX && V)) asm volatile("" : "+v"(id0));
@@ -813,10 +813,11 @@ __global__ __launch_bounds__(256) void apus_route_row_kernel(ApusRouteArgs a, in
 
 /* One row of 16 lanes a token where a lane then has 16 experts at most, else a wave a
  * token. us, 256 experts (wave / row): 8 of 4 groups of 8, sigmoid and bias, 64 / 4095 /
- * 32768 tokens 6.6 / 18.7 / 49.4 -> 6.2 / 9.6 / 22.6; 6 of all, softmax 6.0 / 11.4 / 39.8 ->
+ * 32768 tokens 6.6 / 18.7 / 49.4 -> 6.0 / 9.0 / 22.4; 6 of all, softmax 6.0 / 11.4 / 39.8 ->
  * 5.1 / 5.9 / 15.7. Before both, every score in 64 bits and topk rounds of a wave-wide
- * maximum, 14.3 / - / 121 (scores written) and - / 13.7 / -. Bound by instructions (VALU
- * about 240 a token, four tokens' at once, and the dependences between them); 32768
+ * maximum, 14.3 / - / 121 (scores written) and - / 13.7 / -. Bound by the latency of
+ * dependent steps: 241 vector instructions a token, four tokens' at once, which keep the units
+ * busy half of the time; a wave waits 40 % of its cycles for an operand and 27 % for its turn. 32768
  * tokens' logits take 6.6 us at the rate of a copy. The next round's logits fetched ahead
  * cost a wave a SIMD and 13 to 25 %. */
 hipError_t apus_launch_route(const ApusRouteArgs *a, hipStream_t st) {
@@ -833,7 +834,7 @@ hipError_t apus_launch_route(const ApusRouteArgs *a, hipStream_t st) {
         const int lpg = 16 / a->groups, ne = (per + lpg - 1) / lpg;
         const size_t lds = 4 * (sizeof(RowLds) + a->E * sizeof(double)) + a->E * sizeof(float);
         const bool v = per % (4 * lpg) == 0 && al;
-        /* as many workgroups as are resident, four a CU for a sigmoid's 115 registers, else three;
+        /* as many workgroups as are resident, four a CU for a sigmoid's 113 registers, else three;
          * more would only start over (32768 tokens as above 25.2 us with a workgroup for each
          * 16, 22.6 in rounds; sqrt-softplus 24.5 with four, 20.5 with three) */
         const size_t resident = a->score == APUS_SCORE_SIGMOID ? 1024 : 768;

@@ -420,7 +420,8 @@ int apus_hip_i8_quant_dev(const void *x, int M, int K, int flags, int8_t *codes,
 /* Product of integer codes: out[m, o] = (fp32(sum_k a[m, k] w[o, k]) * ascale[m]) *
  * wscale[o], the sum exact. w [O, K], acodes [M, K], out [M, O] fp32 (BF16-rounded
  * with R_OUT) or BF16 (Y_BF16). K % 4 == 0, K <= 131068, codes 4-byte aligned;
- * K % 16 == 0 and 16-byte alignment take the fast schedules, bit for bit alike. */
+ * K % 16 == 0 and 16-byte alignment take the fast schedules, bit for bit alike; other
+ * shapes take up to 12 times as long (pad K with zeros in both operands). */
 int apus_hip_i8_gemm_dev(const int8_t *w, const float *wscale, const int8_t *acodes,
                          const float *ascale, void *out, int M, int O, int K, int flags);
 /* Linear = i8_quant of x [M, K] (X_BF16: BF16) + product, with a caller workspace
